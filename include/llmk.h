@@ -277,6 +277,48 @@ int llmk_matmul_crossentropy_forward(float* losses, void* logits, llmk_dtype dty
                                      const float* bias, const int* targets, int BT, int C, int Vp, int V,
                                      float dscale, int backward, llmk_math math, void* workspace,
                                      size_t workspace_bytes, void* stream);
+/* ---------------------------------------------- fine-tuning losses (new) */
+/* Losses over logits (rows, Vp) of which the first V columns are live, with
+ * their gradient; fp32 or bf16 logits, Vp % 8 == 0, 16-byte aligned. Both build
+ * on the log-probability of a row's target,
+ *   lp = logits[row, target] - logsumexp(logits[row, :V]).
+ * weights (NULL: all 1) multiplies each row's part of the loss; a row of weight
+ * 0 (prompt, padding) is not read at all: its outputs are 0 and its gradient row
+ * is 0 whatever it, its target or its other inputs hold. A target outside
+ * [0, V) in any other row gives NaN. dlogits (NULL: losses only) receives
+ * dscale times the gradient of the summed losses, 0 on [V, Vp); it may be the
+ * logits buffer itself but not overlap it otherwise. Sums run in a fixed order:
+ * the same inputs give the same bits. The reference has no counterpart (its
+ * only loss is the cross-entropy, gpt2/cuda/cross_entropy.cu:7-32).
+ *
+ * llmk_policy_loss: the clipped policy loss with a KL term. With rho = exp(lp -
+ * old_logps[row]), A = advantages[row] and d = ref_logps[row] - lp,
+ *   losses[row] = w (-min(rho A, clamp(rho, 1 - clip_low, 1 + clip_high) A)
+ *                    + kl_coef (exp(d) - d - 1)).
+ * The gradient is that of the smaller product; where both are equal, that of
+ * rho A. old_logps NULL: rho = 1 with the gradient A (samples of the current
+ * policy). A row of advantage 0 has no policy term. kls (optional) receives
+ * exp(d) - d - 1, logps (optional) lp. ref_logps may be NULL when kl_coef is 0
+ * and kls is NULL. workspace >= llmk_policy_loss_workspace(rows, Vp). */
+size_t llmk_policy_loss_workspace(int rows, int Vp);
+int llmk_policy_loss(float* losses, float* kls, float* logps, void* dlogits, const void* logits, llmk_dtype dtype,
+                     const int* targets, const float* weights, const float* advantages, const float* old_logps,
+                     const float* ref_logps, int rows, int V, int Vp, float clip_low, float clip_high, float kl_coef,
+                     float dscale, void* workspace, size_t workspace_bytes, void* stream);
+/* llmk_preference_loss: 2 * pairs sequences of T rows; sequence p is the
+ * preferred one of pair p, sequence pairs + p the other. With L = sum of w lp
+ * over a sequence, R = ref_logps of the sequence (its sum under the reference
+ * model; NULL: 0) and h = beta ((L - R of p) - (L - R of pairs + p)),
+ *   losses[p] = -(1 - label_smoothing) log sigmoid(h)
+ *               - label_smoothing log sigmoid(-h).
+ * rewards (optional, [2 * pairs]) receives beta (L - R), logps (optional,
+ * [2 * pairs * T]) lp of every row. A sequence without live rows has L = 0.
+ * workspace >= llmk_preference_loss_workspace(pairs, T, Vp). */
+size_t llmk_preference_loss_workspace(int pairs, int T, int Vp);
+int llmk_preference_loss(float* losses, float* rewards, float* logps, void* dlogits, const void* logits,
+                         llmk_dtype dtype, const int* targets, const float* weights, const float* ref_logps, int pairs,
+                         int T, int V, int Vp, float beta, float label_smoothing, float dscale, void* workspace,
+                         size_t workspace_bytes, void* stream);
 /* *out = mean(x[0..n)) on the device, fixed reduction order. */
 int llmk_mean(float* out, const float* x, int n, void* stream);
 
@@ -300,6 +342,38 @@ void llmk_adamw_hparams(float* out8, float lr, float beta1, float beta2, float e
                         float grad_scale);
 int llmk_adamw_device_hparams(float* params, void* params_bf16, const float* grads, float* m, float* v, long long n,
                               const float* hparams, void* stream);
+
+/* ------------------------------------- gradient norm and clipping (new) */
+/* One gradient tensor of n elements, contiguous and aligned to its element
+ * size (n = 0 is allowed): fp32, bf16 or fp16. out / out_dtype say where
+ * llmk_clip_grad_norm writes it: in place (out = data), or to a tensor of the
+ * same type or of fp32. llmk_grad_norm ignores them. */
+typedef struct llmk_tensor {
+  const void* data;
+  void* out;
+  long long n;
+  llmk_dtype dtype;
+  llmk_dtype out_dtype;
+} llmk_tensor;
+/* *norm = |scale| * sqrt(sum of the squares of every element of `count`
+ * tensors), in one launch for up to 1000 tensors and one more for the sum
+ * (sums in 64 bits, in a fixed order). `tensors` is a host array, read during the call. workspace >=
+ * llmk_grad_norm_workspace(). The reference has no counterpart: its trainer
+ * does not clip (gpt2/cuda/gpt2cuda.cu:420-459). */
+size_t llmk_grad_norm_workspace(const llmk_tensor* tensors, int count);
+int llmk_grad_norm(float* norm, const llmk_tensor* tensors, int count, float scale, void* workspace,
+                   size_t workspace_bytes, void* stream);
+/* *norm as above (scale 1), then out = data * min(1, max_norm / (*norm +
+ * 1e-6)) for every tensor, max_norm > 0. A norm that is not finite reaches the
+ * outputs (inf: 0 or NaN, NaN: NaN). No written tensor may overlap another. */
+int llmk_clip_grad_norm(float* norm, const llmk_tensor* tensors, int count, float max_norm, void* workspace,
+                        size_t workspace_bytes, void* stream);
+/* llmk_adamw_device_hparams with gradients clipped on the way in: they are
+ * also multiplied by min(1, max_norm / (*norm + 1e-6)), with *norm in device
+ * memory, the norm of grad_scale * grads (llmk_grad_norm). The gradients are not
+ * rewritten, which saves the pass that llmk_clip_grad_norm would add. */
+int llmk_adamw_clipped(float* params, void* params_bf16, const float* grads, float* m, float* v, long long n,
+                       const float* hparams, const float* norm, float max_norm, void* stream);
 
 #ifdef __cplusplus
 }

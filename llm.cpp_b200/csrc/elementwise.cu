@@ -853,15 +853,23 @@ __global__ void mean_kernel(float* __restrict__ out, const float* __restrict__ x
 // p_bf16 (optional) receives the updated parameters rounded to bf16. The
 // hyperparameters come as kernel arguments, or (hp_dev != nullptr) from
 // device memory, so a captured CUDA graph replays with per-step values.
+// kClip: the gradients are also multiplied by min(1, max_norm / (*norm + 1e-6)),
+// the factor that clips their global norm, so that clipping costs no pass that
+// rewrites them.
 struct AdamHP {
   float lr, b1, b2, eps, wd, inv_c1, inv_c2, grad_scale;
 };
+template <bool kClip>
 __global__ void adamw_kernel(float* __restrict__ p, __nv_bfloat16* __restrict__ p_bf16, const float* __restrict__ g,
                              float* __restrict__ m, float* __restrict__ v, long long n4, AdamHP hp_arg,
-                             const AdamHP* __restrict__ hp_dev) {
+                             const AdamHP* __restrict__ hp_dev, const float* __restrict__ norm, float max_norm) {
   const AdamHP hp = hp_dev ? *hp_dev : hp_arg;
-  const float lr = hp.lr, b1 = hp.b1, b2 = hp.b2, eps = hp.eps, wd = hp.wd, inv_c1 = hp.inv_c1, inv_c2 = hp.inv_c2,
-              grad_scale = hp.grad_scale;
+  const float lr = hp.lr, b1 = hp.b1, b2 = hp.b2, eps = hp.eps, wd = hp.wd, inv_c1 = hp.inv_c1, inv_c2 = hp.inv_c2;
+  float grad_scale = hp.grad_scale;
+  if constexpr (kClip) {
+    const float k = max_norm / (*norm + 1e-6f);
+    grad_scale *= k > 1.f ? 1.f : k;  // a NaN norm reaches the parameters
+  }
   for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < n4;
        i += static_cast<long long>(gridDim.x) * blockDim.x) {
     float4 pp = ld4(p + 4 * i), gg = ld4(g + 4 * i), mm = ld4(m + 4 * i), vv = ld4(v + 4 * i);
@@ -1243,8 +1251,8 @@ int llmk_adamw(float* params, void* params_bf16, const float* grads, float* m, f
   const float inv_c1 = static_cast<float>(1.0 / (1.0 - std::pow(static_cast<double>(beta1), t)));
   const float inv_c2 = static_cast<float>(1.0 / (1.0 - std::pow(static_cast<double>(beta2), t)));
   const AdamHP hp{lr, beta1, beta2, eps, weight_decay, inv_c1, inv_c2, grad_scale};
-  adamw_kernel<<<grid_for(n / 4, 256), 256, 0, static_cast<cudaStream_t>(stream)>>>(
-      params, static_cast<__nv_bfloat16*>(params_bf16), grads, m, v, n / 4, hp, nullptr);
+  adamw_kernel<false><<<grid_for(n / 4, 256), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+      params, static_cast<__nv_bfloat16*>(params_bf16), grads, m, v, n / 4, hp, nullptr, nullptr, 0.f);
   count_launch();
   LLMK_CUDA(cudaGetLastError());
   return LLMK_OK;
@@ -1268,9 +1276,23 @@ int llmk_adamw_device_hparams(float* params, void* params_bf16, const float* gra
   if (!params || !grads || !m || !v || n < 0 || !hparams) return fail(LLMK_ERR_INVALID_ARG, "adamw_device_hparams");
   if (n % 4 || !a16(params) || !a16(params_bf16) || !a16(grads) || !a16(m) || !a16(v) || !a16(hparams))
     return fail(LLMK_ERR_UNSUPPORTED, "adamw_device_hparams: n % 4 == 0 and 16-byte alignment required");
-  adamw_kernel<<<grid_for(n / 4, 256), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+  adamw_kernel<false><<<grid_for(n / 4, 256), 256, 0, static_cast<cudaStream_t>(stream)>>>(
       params, static_cast<__nv_bfloat16*>(params_bf16), grads, m, v, n / 4, AdamHP{},
-      reinterpret_cast<const AdamHP*>(hparams));
+      reinterpret_cast<const AdamHP*>(hparams), nullptr, 0.f);
+  count_launch();
+  LLMK_CUDA(cudaGetLastError());
+  return LLMK_OK;
+}
+
+int llmk_adamw_clipped(float* params, void* params_bf16, const float* grads, float* m, float* v, long long n,
+                       const float* hparams, const float* norm, float max_norm, void* stream) {
+  if (!params || !grads || !m || !v || n < 0 || !hparams || !norm || !(max_norm > 0.f))
+    return fail(LLMK_ERR_INVALID_ARG, "adamw_clipped: null operand, or max_norm not above 0");
+  if (n % 4 || !a16(params) || !a16(params_bf16) || !a16(grads) || !a16(m) || !a16(v) || !a16(hparams))
+    return fail(LLMK_ERR_UNSUPPORTED, "adamw_clipped: n % 4 == 0 and 16-byte alignment required");
+  adamw_kernel<true><<<grid_for(n / 4, 256), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+      params, static_cast<__nv_bfloat16*>(params_bf16), grads, m, v, n / 4, AdamHP{},
+      reinterpret_cast<const AdamHP*>(hparams), norm, max_norm);
   count_launch();
   LLMK_CUDA(cudaGetLastError());
   return LLMK_OK;

@@ -21,6 +21,7 @@
 
 #include "ptx.cuh"
 #include "runtime.h"
+#include "vec8.cuh"
 
 namespace llmk {
 namespace {
@@ -36,36 +37,6 @@ __device__ __forceinline__ void lse_fold(float& m, float& s, float m2, float s2)
   } else {
     s += s2 * __expf(m2 - m);
   }
-}
-
-__device__ __forceinline__ void load8v(const float* p, float* v) {
-  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-__device__ __forceinline__ void load8v(const __nv_bfloat16* p, float* v) {
-  const uint4 u = *reinterpret_cast<const uint4*>(p);
-  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __bfloat1622float2(h[i]);
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
-  }
-}
-__device__ __forceinline__ void store8v(float* p, const float* v) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-}
-__device__ __forceinline__ void store8v(__nv_bfloat16* p, const float* v) {
-  uint4 u;
-  __nv_bfloat162 h[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-  u.x = *reinterpret_cast<uint32_t*>(&h[0]);
-  u.y = *reinterpret_cast<uint32_t*>(&h[1]);
-  u.z = *reinterpret_cast<uint32_t*>(&h[2]);
-  u.w = *reinterpret_cast<uint32_t*>(&h[3]);
-  *reinterpret_cast<uint4*>(p) = u;
 }
 
 // Combine: block = 8 rows, 256 threads; thread (row r = t & 7, group

@@ -44,6 +44,11 @@ class TrainState(C.Structure):
     _fields_ = [("step", C.c_int), ("world", C.c_int), ("shard_idx", C.c_longlong), ("sample_idx", C.c_longlong)]
 
 
+class Tensor(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("out", C.c_void_p), ("n", C.c_longlong), ("dtype", C.c_int),
+                ("out_dtype", C.c_int)]
+
+
 class GPT2Config(C.Structure):
     _fields_ = [("max_seq_len", C.c_int), ("vocab_size", C.c_int), ("padded_vocab_size", C.c_int),
                 ("num_layers", C.c_int), ("num_heads", C.c_int), ("channels", C.c_int)]
@@ -93,6 +98,15 @@ SIGNATURES: dict[str, tuple] = {
     "llmk_adamw": (i32, [vp, vp, vp, vp, vp, i64, f32, f32, f32, f32, f32, i32, f32, vp]),
     "llmk_adamw_hparams": (None, [C.POINTER(f32), f32, f32, f32, f32, f32, i32, f32]),
     "llmk_adamw_device_hparams": (i32, [vp, vp, vp, vp, vp, i64, vp, vp]),
+    "llmk_policy_loss_workspace": (sz, [i32, i32]),
+    "llmk_policy_loss": (i32, [vp, vp, vp, vp, vp, i32, vp, vp, vp, vp, vp, i32, i32, i32, f32, f32, f32, f32, vp, sz,
+                               vp]),
+    "llmk_preference_loss_workspace": (sz, [i32, i32, i32]),
+    "llmk_preference_loss": (i32, [vp, vp, vp, vp, vp, i32, vp, vp, vp, i32, i32, i32, i32, f32, f32, f32, vp, sz, vp]),
+    "llmk_grad_norm_workspace": (sz, [vp, i32]),
+    "llmk_grad_norm": (i32, [vp, vp, i32, f32, vp, sz, vp]),
+    "llmk_clip_grad_norm": (i32, [vp, vp, i32, f32, vp, sz, vp]),
+    "llmk_adamw_clipped": (i32, [vp, vp, vp, vp, vp, i64, vp, vp, f32, vp]),
     # model (include/llmk_gpt2.h)
     "llmk_gpt2_num_parameters": (sz, [C.POINTER(GPT2Config)]),
     "llmk_gpt2_parameter_count": (sz, [vp]),
@@ -213,6 +227,127 @@ def gemm(D, A, B, *, a_trans=False, b_trans=False, math=MATH_BF16, bias=None, re
     ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
     call("llmk_gemm", ptr(D), dtype_code(D), D.stride(0), ptr(A), int(a_trans), A.stride(0), ptr(B), int(b_trans),
          B.stride(0), math, M, N, K, C.byref(ep), ptr(workspace), ws_bytes, stream_ptr(stream))
+
+
+def _ws(workspace) -> tuple[int | None, int]:
+    return (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
+
+
+def _device_of(t) -> int:
+    """Device index of t, which has to be the current CUDA device (the library launches there)."""
+    import torch
+    if not t.is_cuda or t.get_device() != torch.cuda.current_device():
+        raise ValueError(f"expected a tensor on the current CUDA device, got one on {t.device}")
+    return t.get_device()
+
+
+def _check(what: str, dev: int, tensors) -> None:
+    """Each (name, tensor or None, dtype, element count): contiguous, of that type and size, on device dev."""
+    for name, t, dtype, n in tensors:
+        if t is None:
+            continue
+        if t.dtype is not dtype:
+            raise TypeError(f"{what}: {name} must be {dtype}, got {t.dtype}")
+        if t.numel() != n or not t.is_contiguous():
+            raise ValueError(f"{what}: {name} must be contiguous with {n} elements, got {tuple(t.shape)}")
+        if t.get_device() != dev:
+            raise ValueError(f"{what}: {name} is on another device than the logits or parameters")
+
+
+def policy_loss_workspace(rows: int, Vp: int) -> int:
+    """Bytes of scratch memory that policy_loss needs."""
+    return lib().llmk_policy_loss_workspace(rows, Vp)
+
+
+def policy_loss(losses, logits, targets, advantages, *, V=None, weights=None, old_logps=None, ref_logps=None, kls=None,
+                logps=None, dlogits=None, clip_low=0.2, clip_high=0.2, kl_coef=0.0, dscale=1.0, workspace=None,
+                stream=None):
+    """Clipped policy loss over logits (..., Vp), and its gradient when dlogits is given (llmk_policy_loss)."""
+    from torch import float32, int32
+    Vp = logits.shape[-1]
+    rows = logits.numel() // Vp
+    _check("policy_loss", _device_of(logits),
+           (("logits", logits, logits.dtype, rows * Vp), ("dlogits", dlogits, logits.dtype, rows * Vp),
+            ("targets", targets, int32, rows), ("losses", losses, float32, rows),
+            ("advantages", advantages, float32, rows), ("weights", weights, float32, rows),
+            ("old_logps", old_logps, float32, rows), ("ref_logps", ref_logps, float32, rows),
+            ("kls", kls, float32, rows), ("logps", logps, float32, rows)))
+    ws, ws_bytes = _ws(workspace)
+    call("llmk_policy_loss", ptr(losses), ptr(kls), ptr(logps), ptr(dlogits), ptr(logits), dtype_code(logits),
+         ptr(targets), ptr(weights), ptr(advantages), ptr(old_logps), ptr(ref_logps), rows, Vp if V is None else V, Vp,
+         clip_low, clip_high, kl_coef, dscale, ws, ws_bytes, stream_ptr(stream))
+
+
+def preference_loss_workspace(pairs: int, T: int, Vp: int) -> int:
+    """Bytes of scratch memory that preference_loss needs."""
+    return lib().llmk_preference_loss_workspace(pairs, T, Vp)
+
+
+def preference_loss(losses, logits, targets, *, V=None, weights=None, ref_logps=None, rewards=None, logps=None,
+                    dlogits=None, beta=0.1, label_smoothing=0.0, dscale=1.0, workspace=None, stream=None):
+    """Preference loss over losses.numel() pairs of sequences of logits (..., Vp), the preferred ones first, and its
+    gradient when dlogits is given (llmk_preference_loss)."""
+    from torch import float32, int32
+    Vp, pairs = logits.shape[-1], losses.numel()
+    rows = logits.numel() // Vp
+    if pairs == 0 or rows % (2 * pairs):
+        raise ValueError(f"preference_loss: {rows} rows of logits are not {pairs} pairs of sequences")
+    _check("preference_loss", _device_of(logits),
+           (("logits", logits, logits.dtype, rows * Vp), ("dlogits", dlogits, logits.dtype, rows * Vp),
+            ("targets", targets, int32, rows), ("losses", losses, float32, pairs), ("weights", weights, float32, rows),
+            ("ref_logps", ref_logps, float32, 2 * pairs), ("rewards", rewards, float32, 2 * pairs),
+            ("logps", logps, float32, rows)))
+    ws, ws_bytes = _ws(workspace)
+    call("llmk_preference_loss", ptr(losses), ptr(rewards), ptr(logps), ptr(dlogits), ptr(logits), dtype_code(logits),
+         ptr(targets), ptr(weights), ptr(ref_logps), pairs, rows // (2 * pairs), Vp if V is None else V, Vp, beta,
+         label_smoothing, dscale, ws, ws_bytes, stream_ptr(stream))
+
+
+class TensorList:
+    """The gradient tensors that grad_norm and clip_grad_norm run over, and (outs, default: in place) where the
+    clipped ones go. Built once; it keeps the tensors alive."""
+
+    def __init__(self, tensors, outs=None):
+        self.tensors = list(tensors)
+        self.outs = self.tensors if outs is None else list(outs)
+        if len(self.outs) != len(self.tensors) or any(a.numel() != b.numel() for a, b in zip(self.tensors, self.outs)):
+            raise ValueError("TensorList: outs must match tensors")
+        if not all(t.is_contiguous() for t in self.tensors + self.outs):
+            raise ValueError("TensorList: tensors must be contiguous")
+        self.device = _device_of(self.tensors[0]) if self.tensors else -1
+        if any(t.get_device() != self.device for t in self.tensors + self.outs):
+            raise ValueError("TensorList: all tensors must be on one device")
+        self.array = (Tensor * len(self.tensors))(*[Tensor(a.data_ptr(), b.data_ptr(), a.numel(), dtype_code(a),
+                                                           dtype_code(b)) for a, b in zip(self.tensors, self.outs)])
+
+    def __len__(self):
+        return len(self.tensors)
+
+
+def grad_norm_workspace(tensors: TensorList) -> int:
+    """Bytes of scratch memory that grad_norm and clip_grad_norm need."""
+    return lib().llmk_grad_norm_workspace(tensors.array, len(tensors))
+
+
+def grad_norm(norm, tensors: TensorList, *, scale=1.0, workspace=None, stream=None):
+    """norm[0] = |scale| * the 2-norm over all tensors (llmk_grad_norm)."""
+    call("llmk_grad_norm", ptr(norm), tensors.array, len(tensors), scale, *_ws(workspace), stream_ptr(stream))
+
+
+def clip_grad_norm(norm, tensors: TensorList, max_norm, *, workspace=None, stream=None):
+    """norm[0] as grad_norm, and every tensor scaled to a global norm of at most max_norm (llmk_clip_grad_norm)."""
+    call("llmk_clip_grad_norm", ptr(norm), tensors.array, len(tensors), max_norm, *_ws(workspace), stream_ptr(stream))
+
+
+def adamw_clipped(params, grads, m, v, hparams, norm, max_norm, *, params_bf16=None, stream=None):
+    """AdamW with device hyperparameters on gradients clipped by the norm in device memory (llmk_adamw_clipped)."""
+    from torch import bfloat16, float32
+    n = params.numel()
+    _check("adamw_clipped", _device_of(params),
+           (("params", params, float32, n), ("grads", grads, float32, n), ("m", m, float32, n), ("v", v, float32, n),
+            ("params_bf16", params_bf16, bfloat16, n), ("hparams", hparams, float32, 8), ("norm", norm, float32, 1)))
+    call("llmk_adamw_clipped", ptr(params), ptr(params_bf16), ptr(grads), ptr(m), ptr(v), params.numel(), ptr(hparams),
+         ptr(norm), max_norm, stream_ptr(stream))
 
 
 class GPT2:
