@@ -5,12 +5,15 @@
 //   lp = x[target] - max(x) - log(sum_j exp(x_j - max(x))),  j < V,
 // with d(lp)/d(x_j) = [j = target] - softmax(x)_j, so the gradient of either
 // loss is one coefficient c = d(loss)/d(lp) per row times that difference.
-// Three steps, for both:
-//   1. row_slots_kernel: (max, sum exp(x - max)) of every 16 KB slice of a row;
-//   2. one thread per row folds the slices, forms lp and the loss's terms in
-//      64 bits, and leaves the row's (max, c / sum, c, target);
-//   3. row_gradient_kernel: dlogits = [j = target] c - exp(x - max) c / sum.
 // Rows of weight zero (prompts, padding) are not read; their gradient is zero.
+//
+// The policy loss is independent from row to row, so one kernel (row_kernel)
+// reads each row once, keeps it in shared memory while its sum forms, and writes
+// the gradient from there. The preference loss needs the sums over whole
+// sequences before the first gradient: row_kernel leaves each row's (max, sum),
+// preference_pair_kernel forms the losses and every row's coefficient, and
+// row_gradient_kernel streams the logits a second time. Rows too long for
+// shared memory take that second way for the policy loss too.
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -23,15 +26,12 @@
 namespace llmk {
 namespace {
 
-constexpr int kSliceBytes = 16384;
-constexpr int kThreads = 256;
-
 template <typename T>
-constexpr int slice_elems() {
-  return kSliceBytes / static_cast<int>(sizeof(T));
+constexpr int vec_elems() {  // elements of a 16-byte vector
+  return 16 / static_cast<int>(sizeof(T));
 }
 
-// What step 3 needs to know of a row.
+// What the gradient of a row is made of.
 struct __align__(16) RowCoef {
   float max;
   float scale;  // c / sum
@@ -58,64 +58,10 @@ __device__ __forceinline__ double warp_sum_d(double v) {
 // sum 0 (or NaN, when it holds one), not exp(-inf + inf).
 __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.f : m; }
 
-// Step 1. Slots lie in planes, slots[slot * rows + row], so that step 2's
-// neighbouring threads read neighbouring rows.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) row_slots_kernel(float2* __restrict__ slots, const T* __restrict__ logits,
-                                                             const float* __restrict__ weights, int rows, int V, int ld,
-                                                             int nslots) {
-  constexpr int kPer = slice_elems<T>() / (kThreads * 8);
-  __shared__ float red_m[kThreads / 32], red_s[kThreads / 32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long units = static_cast<long long>(rows) * nslots;
-  for (long long u = blockIdx.x; u < units; u += gridDim.x) {
-    const long long row = u / nslots;
-    const int slot = static_cast<int>(u - row * nslots);
-    if (weights && weights[row] == 0.f) continue;
-    const int c0 = slot * slice_elems<T>();
-    const T* x = logits + row * ld + c0;
-    const int n = min(slice_elems<T>(), V - c0);
-    float v[kPer][8];
-    float m = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-      const int e = (k * kThreads + threadIdx.x) * 8;
-      if (e < n) {
-        load8v(x + e, v[k]);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (e + j >= n) v[k][j] = -INFINITY;
-          m = fmaxf(m, v[k][j]);
-        }
-      }
-    }
-    m = warp_max_f(m);
-    if (lane == 0) red_m[warp] = m;
-    __syncthreads();
-    float M = red_m[0];
-#pragma unroll
-    for (int w = 1; w < kThreads / 32; ++w) M = fmaxf(M, red_m[w]);
-    const float ref = finite_max(M);
-    float s = 0.f;
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-      const int e = (k * kThreads + threadIdx.x) * 8;
-      if (e < n) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s += expf(v[k][j] - ref);
-      }
-    }
-    s = warp_sum_f(s);
-    if (lane == 0) red_s[warp] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      float S = 0.f;
-#pragma unroll
-      for (int w = 0; w < kThreads / 32; ++w) S += red_s[w];
-      slots[static_cast<long long>(slot) * rows + row] = make_float2(M, S);
-    }
-  }
-}
+// log of a row's sum of exp(x - max). ex2.approx is 4.9e-8 low on average
+// (measured over 2^22 arguments, whatever their range); over a vocabulary that
+// mean is what remains of its error. The maximum's own term, 1, is exact.
+__device__ __forceinline__ double log_sum(double s) { return log(s + (s - 1.0) * 4.9e-8); }
 
 // max and sum of a row from its slots.
 __device__ __forceinline__ void fold_slots(const float2* __restrict__ slots, long long row, int rows, int nslots, float* m,
@@ -136,7 +82,7 @@ __device__ __forceinline__ void fold_slots(const float2* __restrict__ slots, lon
 template <typename T>
 __device__ __forceinline__ double target_logp(const T* logits, long long row, int ld, int V, int target, float m, double s) {
   if (target < 0 || target >= V) return static_cast<double>(NAN);
-  return static_cast<double>(elem_to_float(logits[row * ld + target])) - static_cast<double>(m) - log(s);
+  return static_cast<double>(elem_to_float(logits[row * ld + target])) - static_cast<double>(m) - log_sum(s);
 }
 
 struct PolicyArgs {
@@ -146,39 +92,36 @@ struct PolicyArgs {
   float clip_low, clip_high, kl_coef, dscale;
 };
 
-// Step 2 of the policy loss. With rho = exp(lp - old), A the advantage and
-// d = ref - lp: loss = w (-min(rho A, clamp(rho) A) + kl_coef (exp(d) - d - 1)).
-// The clipped branch has no gradient; where both are equal (rho inside the
-// bounds, or on one) the unclipped one counts.
-template <typename T>
-__global__ void __launch_bounds__(128) policy_rows_kernel(RowCoef* __restrict__ coefs, const float2* __restrict__ slots,
-                                                          const T* __restrict__ logits, PolicyArgs a, int rows, int V,
-                                                          int ld, int nslots) {
-  const long long row = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (row >= rows) return;
-  const float w = a.weights ? a.weights[row] : 1.f;
-  if (w == 0.f) {
-    a.losses[row] = 0.f;
-    if (a.kls) a.kls[row] = 0.f;
-    if (a.logps) a.logps[row] = 0.f;
-    if (coefs) coefs[row] = RowCoef{0.f, 0.f, 0.f, -1};
-    return;
-  }
-  float m;
-  double s;
-  fold_slots(slots, row, rows, nslots, &m, &s);
-  const int target = a.targets[row];
-  const double lp = target_logp(logits, row, ld, V, target, m, s);
-  const double A = a.advantages[row];
-  const double rho = a.old_logps ? exp(lp - static_cast<double>(a.old_logps[row])) : 1.0;
+// The policy loss of one live row, given lp: writes the row's outputs and
+// returns d(loss)/d(lp) with weight and dscale. With rho = exp(lp - old), A the
+// advantage and d = ref - lp: loss = w (-min(rho A, clamp(rho) A) + kl_coef
+// (exp(d) - d - 1)). The clipped branch has no gradient; where both products are
+// equal (rho inside the bounds, or on one) the unclipped one counts. In 64 bits:
+// exp(d) - d - 1 is a difference of nearly equal numbers for a policy close to
+// its reference, and rho against a bound decides between two gradients.
+struct PolicyRow {
+  float adv, old, ref;
+  int target;
+};
+__device__ __forceinline__ PolicyRow policy_row_load(const PolicyArgs& a, long long row) {
+  PolicyRow r;
+  r.adv = a.advantages[row];
+  r.old = a.old_logps ? a.old_logps[row] : 0.f;
+  r.ref = a.ref_logps ? a.ref_logps[row] : 0.f;
+  r.target = a.targets[row];
+  return r;
+}
+__device__ __forceinline__ double policy_row(const PolicyArgs& a, const PolicyRow& r, long long row, float w, double lp) {
+  const double A = r.adv;
+  const double rho = a.old_logps ? exp(lp - static_cast<double>(r.old)) : 1.0;
   const double lo = 1.0 - static_cast<double>(a.clip_low), hi = 1.0 + static_cast<double>(a.clip_high);
   const double clamped = rho < lo ? lo : (rho > hi ? hi : rho);
   const double s1 = A == 0.0 ? 0.0 : rho * A, s2 = clamped * A;
   double loss = s1 > s2 ? -s2 : -s1;
   double g = s1 > s2 ? 0.0 : -s1;
-  if (!a.old_logps && isnan(lp)) loss = g = lp;
+  if (isnan(lp)) loss = g = lp;  // also where rho does not carry it
   if (a.ref_logps) {
-    const double d = static_cast<double>(a.ref_logps[row]) - lp;
+    const double d = static_cast<double>(r.ref) - lp;
     const double e = expm1(d);
     const double kl = e - d;
     if (a.kls) a.kls[row] = static_cast<float>(kl);
@@ -189,10 +132,387 @@ __global__ void __launch_bounds__(128) policy_rows_kernel(RowCoef* __restrict__ 
   }
   a.losses[row] = static_cast<float>(w * loss);
   if (a.logps) a.logps[row] = static_cast<float>(lp);
-  if (coefs) {
-    const double c = g * w * a.dscale;
-    coefs[row] = RowCoef{finite_max(m), static_cast<float>(c / s), static_cast<float>(c), target};
+  return g * w * a.dscale;
+}
+__device__ __forceinline__ void policy_row_masked(const PolicyArgs& a, long long row) {
+  a.losses[row] = 0.f;
+  if (a.kls) a.kls[row] = 0.f;
+  if (a.logps) a.logps[row] = 0.f;
+}
+
+// exp(d) for a difference d of logits: 2^(d log2 e) with the constant in two
+// parts, so that the product's error does not lean one way.
+__device__ __forceinline__ float exp_diff(float d) { return ex2_approx(fmaf(d, 1.44269502f, d * 1.92596299e-8f)); }
+
+// One 16-byte vector.
+__device__ __forceinline__ void unpack_vec(const uint4& u, float (&v)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
   }
+}
+__device__ __forceinline__ void unpack_vec(const uint4& u, float (&v)[4]) {
+  v[0] = __uint_as_float(u.x); v[1] = __uint_as_float(u.y); v[2] = __uint_as_float(u.z); v[3] = __uint_as_float(u.w);
+}
+template <typename T>
+__device__ __forceinline__ float max_vec(const uint4& u) {
+  if constexpr (sizeof(T) == 2) {
+    auto h = [](const uint32_t& v) { return *reinterpret_cast<const __nv_bfloat162*>(&v); };
+    const __nv_bfloat162 m = __hmax2(__hmax2(h(u.x), h(u.y)), __hmax2(h(u.z), h(u.w)));
+    return fmaxf(__low2float(m), __high2float(m));
+  } else {
+    return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+  }
+}
+template <typename T>
+__device__ __forceinline__ float sum_exp_vec(const uint4& u, float ref) {
+  constexpr int kV = vec_elems<T>();
+  float v[kV];
+  unpack_vec(u, v);
+#pragma unroll
+  for (int j = 0; j < kV; ++j) v[j] = exp_diff(v[j] - ref);
+#pragma unroll
+  for (int n = kV / 2; n > 0; n >>= 1)
+#pragma unroll
+    for (int j = 0; j < n; ++j) v[j] += v[j + n];
+  return v[0];
+}
+
+// A running maximum and the sum of exp(x - m), where m follows the largest
+// value seen, but only once that is more than 10 above it: the terms stay far
+// inside fp32's range, and a rescaling is rare.
+struct RunningSum {
+  float top = -INFINITY, m = -INFINITY, s = 0.f;
+  __device__ __forceinline__ float raise(float vm) {
+    top = fmaxf(top, vm);
+    if (!(vm <= m + 10.f)) {
+      s *= ex2_approx((m - vm) * kLog2e);
+      m = vm;
+    }
+    return finite_max(m);
+  }
+  template <typename T>
+  __device__ __forceinline__ void add(const uint4& u) {
+    const float ref = raise(max_vec<T>(u));
+    s += sum_exp_vec<T>(u, ref);
+  }
+  template <typename T>
+  __device__ __forceinline__ void add(const uint4& u, const uint4& w) {
+    const float ref = raise(fmaxf(max_vec<T>(u), max_vec<T>(w)));
+    s += sum_exp_vec<T>(u, ref) + sum_exp_vec<T>(w, ref);
+  }
+};
+
+// The elements from `keep` on replaced by -inf.
+template <typename T>
+__device__ __forceinline__ uint4 cut_vec(const uint4& u, int keep) {
+  uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 2) {
+      if (2 * i >= keep) w[i] = 0xff80ff80u;
+      else if (2 * i + 1 >= keep) w[i] = (w[i] & 0xffffu) | 0xff800000u;
+    } else {
+      if (i >= keep) w[i] = 0xff800000u;
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// -exp(x - max) scale over a vector: the gradient everywhere but at the target.
+template <typename T>
+struct RowGradient {
+  float max, scale;
+  float k;        // 16-bit output: log2 |scale|, folded into the exponent,
+  uint32_t flip;  // and its sign
+  __device__ __forceinline__ explicit RowGradient(const RowCoef& c) : max(c.max), scale(c.scale), k(0.f), flip(0) {
+    if constexpr (sizeof(T) == 2) {
+      k = log2f(fabsf(scale));
+      flip = scale > 0.f ? 0x80008000u : 0u;
+    }
+  }
+  __device__ __forceinline__ uint4 of(const uint4& u) const {
+    constexpr int kV = vec_elems<T>();
+    float v[kV];
+    unpack_vec(u, v);
+    if constexpr (sizeof(T) == 2) {
+      // rounded to bf16 anyway: one product by log2 e is exact enough
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w[i] = pack_bf16x2(ex2_approx(fmaf(v[2 * i] - max, kLog2e, k)), ex2_approx(fmaf(v[2 * i + 1] - max, kLog2e, k))) ^ flip;
+      return make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = -exp_diff(v[j] - max) * scale;
+      return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    }
+  }
+  // `n` vectors of a row, the first of them number v0, by one warp; the row's
+  // last, partly live vector gets zeros in its padding.
+  __device__ __forceinline__ void store(T* row, const uint4* x, int v0, int n, int V, int lane) const {
+    uint4* d = reinterpret_cast<uint4*>(row) + v0;
+    const int full = min(n, V / vec_elems<T>() - v0);
+    int i = lane;
+    for (; i + 32 < full; i += 64) {
+      const uint4 a = x[i], b = x[i + 32];
+      d[i] = of(a);
+      d[i + 32] = of(b);
+    }
+    if (i < full) d[i] = of(x[i]);
+    if (full < n && lane == 0) {
+      const uint4 o = of(x[full]);
+      uint32_t w[4] = {o.x, o.y, o.z, o.w};
+      const int keep = V % vec_elems<T>();
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(T) == 2) w[j] &= 2 * j >= keep ? 0u : (2 * j + 1 >= keep ? 0x0000ffffu : 0xffffffffu);
+        else w[j] &= j >= keep ? 0u : 0xffffffffu;
+      }
+      d[full] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+  __device__ __forceinline__ float at_target(float x, float c) const { return c - expf(x - max) * scale; }
+};
+
+// Zeros over 16-byte vectors.
+__device__ __forceinline__ void zero_vecs(void* d, int n, int thread, int threads) {
+  for (int i = thread; i < n; i += threads) static_cast<uint4*>(d)[i] = make_uint4(0u, 0u, 0u, 0u);
+}
+
+// A warp's own ring of chunks in shared memory. Lane 0 issues the bulk copies;
+// the warp that reads a chunk is the one that gives its place to the next copy,
+// so a __syncwarp is all the hand-over there is.
+constexpr int kMaxStages = 8;
+struct WarpRing {
+  uint8_t* base;
+  uint64_t* bars;
+  int stages, stage_bytes;
+  int in = 0, out = 0, loading = 0;
+  uint32_t out_phase = 0;
+  unsigned int* status;
+  volatile int* abort_flag;
+  __device__ __forceinline__ void load(const void* src, int bytes, int lane) {
+    if (lane == 0) {
+      mbar_arrive_expect_tx(bars + in, bytes);
+      bulk_load_1d(base + static_cast<size_t>(in) * stage_bytes, src, bytes, bars + in);
+    }
+    if (++in == stages) in = 0;
+    ++loading;
+  }
+  // Waits for the next chunk; false when the wait was given up.
+  __device__ __forceinline__ bool wait(int site) {
+    return __all_sync(0xffffffffu, mbar_wait(bars + out, out_phase, status, abort_flag, site));
+  }
+  __device__ __forceinline__ const uint4* chunk() const {
+    return reinterpret_cast<const uint4*>(base + static_cast<size_t>(out) * stage_bytes);
+  }
+  __device__ __forceinline__ void step() {
+    --loading;
+    if (++out == stages) out = 0, out_phase ^= 1u;
+  }
+  // After a wait that was given up: every copy under way lands before the warp
+  // leaves.
+  __device__ __forceinline__ void drain() {
+    for (; loading > 0; step()) mbar_wait(bars + out, out_phase, status, nullptr, 7);
+  }
+};
+
+enum RowMode { kRowGrad, kRowEval, kRowStats };
+constexpr int kRowWarps = 16;
+constexpr int kRowThreads = 32 * kRowWarps;
+
+// How row_kernel shares rows out. A unit is a row (kRowStats: one of `parts`
+// parts of it) of `vecs` vectors; `group` warps take a unit, each `seg` vectors
+// of it, through its ring in chunks of `sub`.
+struct RowJob {
+  float2* slots;  // kRowStats
+  const float* weights;
+  int rows, V, ld;
+  int parts, vecs, group, seg, sub, stages;
+  unsigned int* status;
+};
+
+// One pass over the rows, one persistent CTA of 16 warps per SM. Groups of
+// warps take one row each: pass A waits for the warp's chunks as they arrive and
+// folds them into its running sum; the group's sums are joined, and its first
+// thread does the row's scalar work in 64 bits; in kRowGrad the chunks stay in
+// shared memory until pass B has written the gradient from them, so the logits
+// are read from memory once, and each chunk's place is then refilled with the
+// group's next row. Masked rows take no chunk. kRowStats leaves (max, sum) of
+// each unit in its slot, planes of `rows`. A wait that is given up (the device
+// status says so) ends the work, not the barriers: the group's warps still meet.
+template <typename T, int kMode>
+__global__ void __launch_bounds__(kRowThreads, 1) row_kernel(T* dlogits, const T* logits, RowJob job, PolicyArgs args) {
+  constexpr int kV = vec_elems<T>();
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint64_t bars[kRowWarps * kMaxStages];
+  __shared__ float2 sums[2][kRowWarps];
+  __shared__ RowCoef coef[kRowWarps];
+  __shared__ int abort_word;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kRowWarps * kMaxStages; ++i) mbar_init(bars + i, 1);
+    abort_word = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  const int G = job.group, group = warp / G, gw = warp - group * G;
+  const int groups = kRowWarps / G;
+  auto meet = [&] {
+    if (G == 1) __syncwarp();
+    else named_barrier_sync(1 + group, G * 32);
+  };
+  WarpRing ring{smem + static_cast<size_t>(warp) * job.stages * job.sub * 16, bars + warp * kMaxStages, job.stages,
+                job.sub * 16};
+  ring.status = job.status;
+  ring.abort_flag = &abort_word;
+  const long long units = static_cast<long long>(job.rows) * job.parts;
+  const long long stride = static_cast<long long>(gridDim.x) * groups;
+  const long long first = static_cast<long long>(group) * gridDim.x + blockIdx.x;
+  const int row_vecs = (job.V + kV - 1) / kV;
+  auto weight_of = [&](long long u) { return u < units && job.weights ? job.weights[u / job.parts] : 1.f; };
+  // this warp's vectors of unit u: the first one's number in the row, and how many
+  auto my_first = [&](long long u) { return static_cast<int>(u % job.parts) * job.vecs + gw * job.seg; };
+  auto my_count = [&](long long u) {
+    const int v0 = static_cast<int>(u % job.parts) * job.vecs;
+    return max(0, min(job.seg, min(job.vecs, row_vecs - v0) - gw * job.seg));
+  };
+
+  // The copies run ahead: (pu, pc) is the next chunk to load.
+  long long pu = first;
+  int pc = 0;
+  float pw = weight_of(pu);
+  auto load_next = [&] {
+    while (pu < units && (pw == 0.f || pc >= my_count(pu))) {
+      pu += stride;
+      pc = 0;
+      pw = weight_of(pu);
+    }
+    if (pu >= units) return;
+    const int n = min(job.sub, my_count(pu) - pc);
+    ring.load(reinterpret_cast<const uint4*>(logits + (pu / job.parts) * job.ld) + my_first(pu) + pc, n * 16, lane);
+    pc += job.sub;
+  };
+  for (int i = 0; i < job.stages; ++i) load_next();
+
+  bool ok = true;
+  int k = 0;  // live units so far
+  float w = weight_of(first);
+  for (long long u = first; u < units; u += stride) {
+    const long long row = u / job.parts;
+    const float weight = w;
+    w = weight_of(u + stride);
+    if (weight == 0.f) {
+      if (kMode == kRowGrad) zero_vecs(dlogits + row * job.ld, job.ld / kV, gw * 32 + lane, G * 32);
+      if (kMode != kRowStats && gw == 0 && lane == 0) policy_row_masked(args, row);
+      continue;
+    }
+    const int v0 = my_first(u), n = my_count(u);
+    PolicyRow r{};
+    float xt = 0.f;
+    if (kMode != kRowStats && gw == 0) {  // ahead of their use
+      r = policy_row_load(args, row);
+      xt = r.target >= 0 && r.target < job.V ? elem_to_float(logits[row * job.ld + r.target]) : NAN;
+    }
+    RunningSum run;
+    const int out0 = ring.out, loading0 = ring.loading;
+    const uint32_t phase0 = ring.out_phase;
+    for (int c = 0; c < n; c += job.sub) {
+      ok = ok && ring.wait(4);
+      const int nc = min(job.sub, n - c);
+      if (!ok) break;
+      const uint4* x = ring.chunk();
+      const int full = min(nc, job.V / kV - v0 - c);
+      int i = lane;
+      for (; i + 32 < full; i += 64) run.add<T>(x[i], x[i + 32]);
+      if (i < full) run.add<T>(x[i]);
+      if (full < nc && lane == 0) run.add<T>(cut_vec<T>(x[full], job.V % kV));
+      ring.step();
+      if (kMode != kRowGrad) {
+        __syncwarp();
+        load_next();
+      }
+    }
+    const float m = warp_max_f(run.top);
+    const float s = warp_sum_f(run.s * exp_diff(run.m - finite_max(m)));
+    // Two sets of sums: a set is rewritten two rows on, and between lies a
+    // meeting that the group's first warp reaches only after reading it.
+    if (lane == 0) sums[k & 1][warp] = make_float2(m, s);
+    meet();
+    if (gw == 0) {
+      const float2 p = lane < G ? sums[k & 1][warp + lane] : make_float2(-INFINITY, 0.f);
+      const float M = warp_max_f(p.x);
+      const float ref = finite_max(M);
+      const double S = warp_sum_d(static_cast<double>(p.y * expf(p.x - ref)));
+      if (lane == 0) {
+        if (kMode == kRowStats) {
+          job.slots[(u % job.parts) * job.rows + row] = make_float2(M, static_cast<float>(S));
+        } else {
+          const double c = policy_row(args, r, row, weight, static_cast<double>(xt) - static_cast<double>(M) - log_sum(S));
+          if (kMode == kRowGrad) coef[warp] = RowCoef{ref, static_cast<float>(c / S), static_cast<float>(c), r.target};
+        }
+      }
+    }
+    ++k;
+    if (kMode == kRowGrad) {
+      meet();
+      const RowCoef rc = coef[group * G];
+      T* d = dlogits + row * job.ld;
+      // back over the same chunks
+      ring.out = out0, ring.out_phase = phase0, ring.loading = loading0;
+      if (ok && rc.c == 0.f) {
+        zero_vecs(reinterpret_cast<uint4*>(d) + v0, n, lane, 32);
+        for (int c = 0; c < n; c += job.sub) {
+          ring.step();
+          load_next();
+        }
+      } else if (ok) {
+        const RowGradient<T> g(rc);
+        float at = 0.f;
+        bool target_here = false;
+        for (int c = 0; c < n; c += job.sub) {
+          const int nc = min(job.sub, n - c);
+          g.store(d, ring.chunk(), v0 + c, nc, job.V, lane);
+          const int t = rc.target - (v0 + c) * kV;
+          if (t >= 0 && t < nc * kV && rc.target < job.V) {
+            target_here = true;
+            at = g.at_target(elem_to_float(reinterpret_cast<const T*>(ring.chunk())[t]), rc.c);
+          }
+          ring.step();
+          __syncwarp();
+          load_next();
+        }
+        if (target_here && lane == 0) elem_store(d + rc.target, at);
+      }
+      if (gw == G - 1) zero_vecs(reinterpret_cast<uint4*>(d) + row_vecs, job.ld / kV - row_vecs, lane, 32);
+    }
+  }
+  ring.drain();
+}
+
+// The policy loss from slots, one thread a row (rows too long for row_kernel to
+// keep).
+template <typename T>
+__global__ void __launch_bounds__(128) policy_rows_kernel(RowCoef* __restrict__ coefs, const float2* __restrict__ slots,
+                                                          const T* __restrict__ logits, PolicyArgs a, int rows, int V,
+                                                          int ld, int nslots) {
+  const long long row = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (row >= rows) return;
+  const float w = a.weights ? a.weights[row] : 1.f;
+  if (w == 0.f) {
+    policy_row_masked(a, row);
+    coefs[row] = RowCoef{0.f, 0.f, 0.f, -1};
+    return;
+  }
+  float m;
+  double s;
+  fold_slots(slots, row, rows, nslots, &m, &s);
+  const PolicyRow r = policy_row_load(a, row);
+  const double c = policy_row(a, r, row, w, target_logp(logits, row, ld, V, r.target, m, s));
+  coefs[row] = RowCoef{finite_max(m), static_cast<float>(c / s), static_cast<float>(c), r.target};
 }
 
 struct PreferenceArgs {
@@ -276,62 +596,85 @@ __global__ void __launch_bounds__(kPairThreads) preference_pair_kernel(RowCoef* 
   }
 }
 
-// Step 3. dlogits may be the logits: every thread writes only what it read.
+// The gradient from each row's coefficient: a persistent pass, each warp taking
+// units of up to `sub` vectors of a row through its own ring. Rows of coefficient
+// 0 are written without being read. dlogits may be the logits: a unit is read
+// whole before any of it is written, and by its own warp only.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) row_gradient_kernel(T* dlogits, const T* logits,
-                                                                const RowCoef* __restrict__ coefs, int rows, int V,
-                                                                int ld, int nslots) {
-  constexpr int kPer = slice_elems<T>() / (kThreads * 8);
-  const long long units = static_cast<long long>(rows) * nslots;
-  for (long long u = blockIdx.x; u < units; u += gridDim.x) {
-    const long long row = u / nslots;
-    const int c0 = static_cast<int>(u - row * nslots) * slice_elems<T>();
-    const int n = min(slice_elems<T>(), ld - c0);
-    const RowCoef rc = coefs[row];
-    const T* x = logits + row * ld + c0;
-    T* d = dlogits + row * ld + c0;
+__global__ void __launch_bounds__(kRowThreads, 1) row_gradient_kernel(T* dlogits, const T* logits,
+                                                                      const RowCoef* __restrict__ coefs, int rows, int V,
+                                                                      int ld, int sub, int stages, unsigned int* status) {
+  constexpr int kV = vec_elems<T>();
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint64_t bars[kRowWarps * kMaxStages];
+  __shared__ int abort_word;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kRowWarps * kMaxStages; ++i) mbar_init(bars + i, 1);
+    abort_word = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  WarpRing ring{smem + static_cast<size_t>(warp) * stages * sub * 16, bars + warp * kMaxStages, stages, sub * 16};
+  ring.status = status;
+  ring.abort_flag = &abort_word;
+  const int row_vecs = ld / kV, upr = (row_vecs + sub - 1) / sub;
+  const long long units = static_cast<long long>(rows) * upr;
+  const long long stride = static_cast<long long>(gridDim.x) * kRowWarps;
+  const long long first = static_cast<long long>(warp) * gridDim.x + blockIdx.x;
+  auto coef_of = [&](long long u) { return u < units ? coefs[u / upr] : RowCoef{0.f, 0.f, 0.f, -1}; };
+  auto first_vec = [&](long long u) { return static_cast<int>(u % upr) * sub; };
+  long long pu = first;
+  float pc = coef_of(pu).c;
+  auto load_next = [&] {
+    while (pu < units && pc == 0.f) pu += stride, pc = coef_of(pu).c;
+    if (pu >= units) return;
+    const int v0 = first_vec(pu);
+    ring.load(reinterpret_cast<const uint4*>(logits + (pu / upr) * ld) + v0, min(sub, row_vecs - v0) * 16, lane);
+    pu += stride;
+    pc = coef_of(pu).c;
+  };
+  for (int i = 0; i < stages; ++i) load_next();
+  bool ok = true;
+  RowCoef next = coef_of(first);
+  for (long long u = first; u < units; u += stride) {
+    const RowCoef rc = next;
+    next = coef_of(u + stride);
+    const int v0 = first_vec(u), n = min(sub, row_vecs - v0);
+    T* d = dlogits + (u / upr) * ld;
     if (rc.c == 0.f) {
-      const float zero[8] = {};
-#pragma unroll
-      for (int k = 0; k < kPer; ++k) {
-        const int e = (k * kThreads + threadIdx.x) * 8;
-        if (e < n) store8v(d + e, zero);
-      }
+      zero_vecs(reinterpret_cast<uint4*>(d) + v0, n, lane, 32);
       continue;
     }
-    float v[kPer][8];
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-      const int e = (k * kThreads + threadIdx.x) * 8;
-      if (e < n) load8v(x + e, v[k]);
-    }
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-      const int e = (k * kThreads + threadIdx.x) * 8, c = c0 + e;
-      if (e < n) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          float g = -expf(v[k][j] - rc.max) * rc.scale;
-          if (c + j == rc.target) g += rc.c;
-          v[k][j] = c + j < V ? g : 0.f;
-        }
-        store8v(d + e, v[k]);
-      }
+    ok = ok && ring.wait(6);
+    if (ok) {
+      const RowGradient<T> g(rc);
+      const int live = min(n, (V + kV - 1) / kV - v0);  // may be negative: padding only
+      if (live > 0) g.store(d, ring.chunk(), v0, live, V, lane);
+      zero_vecs(reinterpret_cast<uint4*>(d) + v0 + max(live, 0), n - max(live, 0), lane, 32);
+      const int t = rc.target - v0 * kV;
+      const bool here = t >= 0 && t < n * kV;
+      const float x = here ? elem_to_float(reinterpret_cast<const T*>(ring.chunk())[t]) : 0.f;
+      __syncwarp();
+      if (here && rc.target < V && lane == 0) elem_store(d + rc.target, g.at_target(x, rc.c));
+      ring.step();
+      load_next();
     }
   }
+  ring.drain();
 }
 
-template <typename T>
-int slots_of(int cols) {
-  return (cols + slice_elems<T>() - 1) / slice_elems<T>();
+// Units a row is cut into when only its sum is wanted: enough that every SM has
+// a few, at least 256 vectors of bf16 each.
+int parts_of(long long rows, int V) {
+  const long long want = (4LL * num_sms() + rows - 1) / rows;
+  return static_cast<int>(std::max(1LL, std::min<long long>({want, 16, (V + 2047) / 2048})));
 }
 
-int grid_of(long long units) { return static_cast<int>(std::min<long long>(units, num_sms() * 8LL)); }
-
-// Scratch of `rows` rows of `Vp` columns: the slot planes (at the fp32 slot
-// count, the larger one), then one RowCoef per row.
+// Scratch of `rows` rows of `Vp` columns: the slot planes, then one RowCoef per
+// row.
 size_t slots_bytes(long long rows, int Vp) {
-  return (static_cast<size_t>(slots_of<float>(Vp)) * rows * sizeof(float2) + 15) / 16 * 16;
+  return (static_cast<size_t>(parts_of(rows, Vp)) * rows * sizeof(float2) + 15) / 16 * 16;
 }
 size_t loss_workspace(long long rows, int Vp) { return slots_bytes(rows, Vp) + static_cast<size_t>(rows) * sizeof(RowCoef); }
 
@@ -353,21 +696,89 @@ int check_rows(const char* what, void* dlogits, const void* logits, llmk_dtype d
   return LLMK_OK;
 }
 
-template <typename T>
-int launch_slots(float2* slots, const void* logits, const float* weights, int rows, int V, int Vp, cudaStream_t s) {
-  const int n = slots_of<T>(V);
-  row_slots_kernel<T><<<grid_of(static_cast<long long>(rows) * n), kThreads, 0, s>>>(
-      slots, static_cast<const T*>(logits), weights, rows, V, Vp, n);
+// Opts a kernel into its dynamic shared memory, once per device.
+template <typename K>
+int allow_smem(K kernel, size_t bytes, bool (&done)[64]) {
+  int dev = 0;
+  LLMK_CUDA(cudaGetDevice(&dev));
+  if (dev < 64 && done[dev]) return LLMK_OK;
+  LLMK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+  if (dev < 64) done[dev] = true;
+  return LLMK_OK;
+}
+
+int div_up(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
+
+// Bytes of shared memory that a warp's ring may take: 16 of them and the static
+// part fit the 227 KB of an SM.
+constexpr int kWarpRingBytes = 14336;
+
+// Fills in group, seg, sub and stages for units of job.vecs vectors; false when
+// `keep` is asked (a unit stays in its group's rings) and it does not fit.
+bool share_out(RowJob* job, bool keep) {
+  const int warp_vecs = kWarpRingBytes / 16;
+  const long long units = static_cast<long long>(job->rows) * job->parts;
+  // the fewest warps a unit fits, so that groups work on rows of their own and
+  // one's barriers are hidden by the others, ...
+  int group = 1;
+  while (group < kRowWarps && job->vecs > group * warp_vecs) group *= 2;
+  if (keep && job->vecs > group * warp_vecs) return false;
+  // ... but no fewer than it takes to keep all warps busy with few units
+  while (group < kRowWarps && units * group < static_cast<long long>(num_sms()) * kRowWarps && job->vecs > 32 * group) group *= 2;
+  job->group = group;
+  job->seg = div_up(job->vecs, group);
+  const int chunks = std::max(1, std::min(div_up(job->seg, 256), 4));
+  job->sub = std::min(div_up(div_up(job->seg, chunks), 32) * 32, 256);
+  job->stages = std::min(kMaxStages, warp_vecs / job->sub);
+  return !keep || job->stages * job->sub >= job->seg;
+}
+
+template <typename T, int kMode>
+int launch_rows(void* dlogits, const void* logits, const RowJob& job, const PolicyArgs& a, cudaStream_t s) {
+  static bool done[64] = {};
+  LLMK_TRY(allow_smem(row_kernel<T, kMode>, kRowWarps * kWarpRingBytes, done));
+  const long long units = static_cast<long long>(job.rows) * job.parts;
+  const size_t smem = static_cast<size_t>(kRowWarps) * job.stages * job.sub * 16;
+  row_kernel<T, kMode><<<static_cast<int>(std::min<long long>(units, num_sms())), kRowThreads, smem, s>>>(
+      static_cast<T*>(dlogits), static_cast<const T*>(logits), job, a);
   count_launch();
   LLMK_CUDA(cudaGetLastError());
   return LLMK_OK;
 }
 
 template <typename T>
+RowJob row_job(const float* weights, int rows, int V, int Vp) {
+  RowJob job{};
+  job.weights = weights;
+  job.rows = rows, job.V = V, job.ld = Vp;
+  job.parts = 1;
+  job.vecs = div_up(V, vec_elems<T>());
+  job.status = device_status_ptr();
+  return job;
+}
+
+// Slots of every live row; returns the number of planes through *nslots.
+template <typename T>
+int launch_slots(float2* slots, int* nslots, const void* logits, const float* weights, int rows, int V, int Vp, cudaStream_t s) {
+  RowJob job = row_job<T>(weights, rows, V, Vp);
+  const int all = job.vecs;
+  job.slots = slots;
+  job.vecs = div_up(all, parts_of(rows, V));
+  job.parts = *nslots = div_up(all, job.vecs);  // rounding up may leave the last part empty
+  share_out(&job, false);
+  return launch_rows<T, kRowStats>(nullptr, logits, job, PolicyArgs{}, s);
+}
+
+template <typename T>
 int launch_gradient(void* dlogits, const void* logits, const RowCoef* coefs, int rows, int V, int Vp, cudaStream_t s) {
-  const int n = slots_of<T>(Vp);
-  row_gradient_kernel<T><<<grid_of(static_cast<long long>(rows) * n), kThreads, 0, s>>>(
-      static_cast<T*>(dlogits), static_cast<const T*>(logits), coefs, rows, V, Vp, n);
+  static bool done[64] = {};
+  LLMK_TRY(allow_smem(row_gradient_kernel<T>, kRowWarps * kWarpRingBytes, done));
+  const int vecs = Vp / vec_elems<T>(), chunks = div_up(vecs, 224), sub = div_up(div_up(vecs, chunks), 32) * 32;
+  const int stages = std::min(kMaxStages, kWarpRingBytes / (sub * 16));
+  const long long units = static_cast<long long>(rows) * div_up(vecs, sub);
+  row_gradient_kernel<T><<<static_cast<int>(std::min<long long>(units, num_sms())), kRowThreads,
+                           static_cast<size_t>(kRowWarps) * stages * sub * 16, s>>>(
+      static_cast<T*>(dlogits), static_cast<const T*>(logits), coefs, rows, V, Vp, sub, stages, device_status_ptr());
   count_launch();
   LLMK_CUDA(cudaGetLastError());
   return LLMK_OK;
@@ -376,14 +787,21 @@ int launch_gradient(void* dlogits, const void* logits, const RowCoef* coefs, int
 template <typename T>
 int policy_loss(void* dlogits, const void* logits, const PolicyArgs& a, int rows, int V, int Vp, void* workspace,
                 cudaStream_t s) {
+  RowJob job = row_job<T>(a.weights, rows, V, Vp);
+  if (!dlogits) {
+    share_out(&job, false);
+    return launch_rows<T, kRowEval>(nullptr, logits, job, a, s);
+  }
+  if (share_out(&job, true)) return launch_rows<T, kRowGrad>(dlogits, logits, job, a, s);
   auto* slots = static_cast<float2*>(workspace);
-  auto* coefs = dlogits ? reinterpret_cast<RowCoef*>(static_cast<char*>(workspace) + slots_bytes(rows, Vp)) : nullptr;
-  LLMK_TRY(launch_slots<T>(slots, logits, a.weights, rows, V, Vp, s));
-  policy_rows_kernel<T><<<static_cast<int>((rows + 127LL) / 128), 128, 0, s>>>(coefs, slots, static_cast<const T*>(logits), a, rows, V, Vp,
-                                                           slots_of<T>(V));
+  auto* coefs = reinterpret_cast<RowCoef*>(static_cast<char*>(workspace) + slots_bytes(rows, Vp));
+  int nslots = 0;
+  LLMK_TRY(launch_slots<T>(slots, &nslots, logits, a.weights, rows, V, Vp, s));
+  policy_rows_kernel<T><<<div_up(rows, 128), 128, 0, s>>>(coefs, slots, static_cast<const T*>(logits), a, rows, V, Vp,
+                                                          nslots);
   count_launch();
   LLMK_CUDA(cudaGetLastError());
-  return dlogits ? launch_gradient<T>(dlogits, logits, coefs, rows, V, Vp, s) : LLMK_OK;
+  return launch_gradient<T>(dlogits, logits, coefs, rows, V, Vp, s);
 }
 
 template <typename T>
@@ -392,9 +810,10 @@ int preference_loss(void* dlogits, const void* logits, const PreferenceArgs& a, 
   const int rows = 2 * pairs * Tlen;
   auto* slots = static_cast<float2*>(workspace);
   auto* coefs = dlogits ? reinterpret_cast<RowCoef*>(static_cast<char*>(workspace) + slots_bytes(rows, Vp)) : nullptr;
-  LLMK_TRY(launch_slots<T>(slots, logits, a.weights, rows, V, Vp, s));
+  int nslots = 0;
+  LLMK_TRY(launch_slots<T>(slots, &nslots, logits, a.weights, rows, V, Vp, s));
   preference_pair_kernel<T><<<pairs, kPairThreads, 0, s>>>(coefs, slots, static_cast<const T*>(logits), a, pairs, Tlen, V,
-                                                           Vp, slots_of<T>(V));
+                                                           Vp, nslots);
   count_launch();
   LLMK_CUDA(cudaGetLastError());
   return dlogits ? launch_gradient<T>(dlogits, logits, coefs, rows, V, Vp, s) : LLMK_OK;
