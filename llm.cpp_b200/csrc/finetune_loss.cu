@@ -31,6 +31,13 @@ constexpr int vec_elems() {  // elements of a 16-byte vector
   return 16 / static_cast<int>(sizeof(T));
 }
 
+// The maximum of a row, or of part of one, and the sum of exp(x - max). The sum
+// is a double: what corrects it is less than half a step of fp32.
+struct __align__(16) RowSum {
+  double s;
+  float m;
+};
+
 // What the gradient of a row is made of.
 struct __align__(16) RowCoef {
   float max;
@@ -58,21 +65,16 @@ __device__ __forceinline__ double warp_sum_d(double v) {
 // sum 0 (or NaN, when it holds one), not exp(-inf + inf).
 __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.f : m; }
 
-// log of a row's sum of exp(x - max). ex2.approx is 4.9e-8 low on average
-// (measured over 2^22 arguments, whatever their range); over a vocabulary that
-// mean is what remains of its error. The maximum's own term, 1, is exact.
-__device__ __forceinline__ double log_sum(double s) { return log(s + (s - 1.0) * 4.9e-8); }
-
 // max and sum of a row from its slots.
-__device__ __forceinline__ void fold_slots(const float2* __restrict__ slots, long long row, int rows, int nslots, float* m,
+__device__ __forceinline__ void fold_slots(const RowSum* __restrict__ slots, long long row, int rows, int nslots, float* m,
                                            double* s) {
   float M = -INFINITY;
-  for (int k = 0; k < nslots; ++k) M = fmaxf(M, slots[static_cast<long long>(k) * rows + row].x);
+  for (int k = 0; k < nslots; ++k) M = fmaxf(M, slots[static_cast<long long>(k) * rows + row].m);
   const float ref = finite_max(M);
   double S = 0.0;
   for (int k = 0; k < nslots; ++k) {
-    const float2 p = slots[static_cast<long long>(k) * rows + row];
-    S += static_cast<double>(p.y * expf(p.x - ref));
+    const RowSum p = slots[static_cast<long long>(k) * rows + row];
+    S += p.s * exp(static_cast<double>(p.m - ref));
   }
   *m = M;
   *s = S;
@@ -82,7 +84,7 @@ __device__ __forceinline__ void fold_slots(const float2* __restrict__ slots, lon
 template <typename T>
 __device__ __forceinline__ double target_logp(const T* logits, long long row, int ld, int V, int target, float m, double s) {
   if (target < 0 || target >= V) return static_cast<double>(NAN);
-  return static_cast<double>(elem_to_float(logits[row * ld + target])) - static_cast<double>(m) - log_sum(s);
+  return static_cast<double>(elem_to_float(logits[row * ld + target])) - static_cast<double>(m) - log(s);
 }
 
 struct PolicyArgs {
@@ -166,45 +168,6 @@ __device__ __forceinline__ float max_vec(const uint4& u) {
     return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
   }
 }
-template <typename T>
-__device__ __forceinline__ float sum_exp_vec(const uint4& u, float ref) {
-  constexpr int kV = vec_elems<T>();
-  float v[kV];
-  unpack_vec(u, v);
-#pragma unroll
-  for (int j = 0; j < kV; ++j) v[j] = exp_diff(v[j] - ref);
-#pragma unroll
-  for (int n = kV / 2; n > 0; n >>= 1)
-#pragma unroll
-    for (int j = 0; j < n; ++j) v[j] += v[j + n];
-  return v[0];
-}
-
-// A running maximum and the sum of exp(x - m), where m follows the largest
-// value seen, but only once that is more than 10 above it: the terms stay far
-// inside fp32's range, and a rescaling is rare.
-struct RunningSum {
-  float top = -INFINITY, m = -INFINITY, s = 0.f;
-  __device__ __forceinline__ float raise(float vm) {
-    top = fmaxf(top, vm);
-    if (!(vm <= m + 10.f)) {
-      s *= ex2_approx((m - vm) * kLog2e);
-      m = vm;
-    }
-    return finite_max(m);
-  }
-  template <typename T>
-  __device__ __forceinline__ void add(const uint4& u) {
-    const float ref = raise(max_vec<T>(u));
-    s += sum_exp_vec<T>(u, ref);
-  }
-  template <typename T>
-  __device__ __forceinline__ void add(const uint4& u, const uint4& w) {
-    const float ref = raise(fmaxf(max_vec<T>(u), max_vec<T>(w)));
-    s += sum_exp_vec<T>(u, ref) + sum_exp_vec<T>(w, ref);
-  }
-};
-
 // The elements from `keep` on replaced by -inf.
 template <typename T>
 __device__ __forceinline__ uint4 cut_vec(const uint4& u, int keep) {
@@ -220,6 +183,97 @@ __device__ __forceinline__ uint4 cut_vec(const uint4& u, int keep) {
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
+
+// Sum of exp(x - ref) over a vector; *first: its first element's term.
+template <typename T>
+__device__ __forceinline__ float sum_exp_vec(const uint4& u, float ref, float* first) {
+  constexpr int kV = vec_elems<T>();
+  float v[kV];
+  unpack_vec(u, v);
+#pragma unroll
+  for (int j = 0; j < kV; ++j) v[j] = exp_diff(v[j] - ref);
+  *first = v[0];
+#pragma unroll
+  for (int n = kV / 2; n > 0; n >>= 1)
+#pragma unroll
+    for (int j = 0; j < n; ++j) v[j] += v[j + n];
+  return v[0];
+}
+template <typename T>
+__device__ __forceinline__ float first_elem(const uint4& u) {
+  return __uint_as_float(sizeof(T) == 2 ? u.x << 16 : u.x);
+}
+
+// A running maximum and the sum of exp(x - m), where m follows the largest
+// value seen, but only once that is more than 10 above it: the terms stay far
+// inside fp32's range, and a rescaling is rare.
+// ex2.approx is 5e-8 low on average, a little more or less by the spread of the
+// logits (measured), and a sum over a vocabulary keeps that mean while the
+// rounding errors cancel; a preference loss adds such sums over a thousand
+// positions. So one term in 16 is also computed by expf (6e-9 high on average),
+// and the sum is corrected by what those terms differ by: the mean error of a
+// row's log-probability falls from 5e-8 to 3e-9 for one more instruction per
+// element.
+struct RunningSum {
+  float top = -INFINITY, m = -INFINITY, s = 0.f;
+  float part = 0.f, off = 0.f;  // the terms computed twice: their sum, and what it lacks
+  __device__ __forceinline__ float raise(float vm) {
+    top = fmaxf(top, vm);
+    if (!(vm <= m + 10.f)) {
+      const float f = ex2_approx((m - vm) * kLog2e);
+      s *= f, part *= f, off *= f;
+      m = vm;
+    }
+    return finite_max(m);
+  }
+  __device__ __forceinline__ void twice(float x, float ref, float e) {
+    part += e;
+    off += expf(x - ref) - e;
+  }
+  template <typename T>
+  __device__ __forceinline__ void add(const uint4& u) {
+    const float ref = raise(max_vec<T>(u));
+    float e;
+    s += sum_exp_vec<T>(u, ref, &e);
+    twice(first_elem<T>(u), ref, e);
+  }
+  template <typename T>
+  __device__ __forceinline__ void add(const uint4& u, const uint4& w) {
+    const float ref = raise(fmaxf(max_vec<T>(u), max_vec<T>(w)));
+    float e, unused;
+    s += sum_exp_vec<T>(u, ref, &e) + sum_exp_vec<T>(w, ref, &unused);
+    if (sizeof(T) == 2) twice(first_elem<T>(u), ref, e);
+  }
+  // fp32 vectors are half as long
+  template <typename T>
+  __device__ __forceinline__ void add(const uint4& a, const uint4& b, const uint4& c, const uint4& d) {
+    const float ref = raise(fmaxf(fmaxf(max_vec<T>(a), max_vec<T>(b)), fmaxf(max_vec<T>(c), max_vec<T>(d))));
+    float e, unused;
+    s += (sum_exp_vec<T>(a, ref, &e) + sum_exp_vec<T>(b, ref, &unused)) +
+         (sum_exp_vec<T>(c, ref, &unused) + sum_exp_vec<T>(d, ref, &unused));
+    twice(first_elem<T>(a), ref, e);
+  }
+  // The warp's vectors x[0, full), and x[full] cut after `keep` elements when there is one.
+  template <typename T>
+  __device__ __forceinline__ void add_all(const uint4* x, int full, bool partial, int keep, int lane) {
+    int i = lane;
+    if (sizeof(T) == 4)
+      for (; i + 96 < full; i += 128) add<T>(x[i], x[i + 32], x[i + 64], x[i + 96]);
+    for (; i + 32 < full; i += 64) add<T>(x[i], x[i + 32]);
+    if (i < full) add<T>(x[i]);
+    if (partial && lane == 0) add<T>(cut_vec<T>(x[full], keep));
+  }
+  // The warp's maximum and sum of exp(x - maximum); the maximum's own term is
+  // exactly 1 and needs no correction.
+  __device__ __forceinline__ RowSum join() const {
+    const float M = warp_max_f(top);
+    // one factor for all of the lane's terms: expf's error would not cancel
+    const double f = exp(static_cast<double>(m - finite_max(M)));
+    const double S = warp_sum_d(static_cast<double>(s) * f);
+    const float P = warp_sum_f(part * static_cast<float>(f)), D = warp_sum_f(off * static_cast<float>(f));
+    return RowSum{P > 0.f ? S + (S - 1.0) * (static_cast<double>(D / P) - 6e-9) : S, M};
+  }
+};
 
 // -exp(x - max) scale over a vector: the gradient everywhere but at the target.
 template <typename T>
@@ -320,6 +374,24 @@ struct WarpRing {
   }
 };
 
+// A place in a grid of rows x parts, walked with a fixed stride: no division on
+// the way.
+struct UnitWalk {
+  long long row;
+  int part;
+  int rows, parts, step_part;
+  long long step_row;
+  __device__ __forceinline__ UnitWalk(long long first, long long stride, int rows_, int parts_)
+      : row(first / parts_), part(static_cast<int>(first % parts_)), rows(rows_), parts(parts_),
+        step_part(static_cast<int>(stride % parts_)), step_row(stride / parts_) {}
+  __device__ __forceinline__ bool valid() const { return row < rows; }
+  __device__ __forceinline__ void next() {
+    row += step_row;
+    part += step_part;
+    if (part >= parts) part -= parts, ++row;
+  }
+};
+
 enum RowMode { kRowGrad, kRowEval, kRowStats };
 constexpr int kRowWarps = 16;
 constexpr int kRowThreads = 32 * kRowWarps;
@@ -328,7 +400,7 @@ constexpr int kRowThreads = 32 * kRowWarps;
 // parts of it) of `vecs` vectors; `group` warps take a unit, each `seg` vectors
 // of it, through its ring in chunks of `sub`.
 struct RowJob {
-  float2* slots;  // kRowStats
+  RowSum* slots;  // kRowStats
   const float* weights;
   int rows, V, ld;
   int parts, vecs, group, seg, sub, stages;
@@ -349,7 +421,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) row_kernel(T* dlogits, const T
   constexpr int kV = vec_elems<T>();
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t bars[kRowWarps * kMaxStages];
-  __shared__ float2 sums[2][kRowWarps];
+  __shared__ RowSum sums[2][kRowWarps];
   __shared__ RowCoef coef[kRowWarps];
   __shared__ int abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -369,42 +441,44 @@ __global__ void __launch_bounds__(kRowThreads, 1) row_kernel(T* dlogits, const T
                 job.sub * 16};
   ring.status = job.status;
   ring.abort_flag = &abort_word;
-  const long long units = static_cast<long long>(job.rows) * job.parts;
   const long long stride = static_cast<long long>(gridDim.x) * groups;
-  const long long first = static_cast<long long>(group) * gridDim.x + blockIdx.x;
   const int row_vecs = (job.V + kV - 1) / kV;
-  auto weight_of = [&](long long u) { return u < units && job.weights ? job.weights[u / job.parts] : 1.f; };
-  // this warp's vectors of unit u: the first one's number in the row, and how many
-  auto my_first = [&](long long u) { return static_cast<int>(u % job.parts) * job.vecs + gw * job.seg; };
-  auto my_count = [&](long long u) {
-    const int v0 = static_cast<int>(u % job.parts) * job.vecs;
-    return max(0, min(job.seg, min(job.vecs, row_vecs - v0) - gw * job.seg));
+  UnitWalk at(static_cast<long long>(group) * gridDim.x + blockIdx.x, stride, job.rows, kMode == kRowStats ? job.parts : 1);
+  UnitWalk ahead = at;  // the unit whose chunks are loaded next
+  auto weight_of = [&](const UnitWalk& u) { return u.valid() && job.weights ? job.weights[u.row] : 1.f; };
+  // this warp's vectors of a unit: the first one's number in the row, and how many
+  auto my_first = [&](const UnitWalk& u) { return u.part * job.vecs + gw * job.seg; };
+  auto my_count = [&](const UnitWalk& u) {
+    return max(0, min(job.seg, min(job.vecs, row_vecs - u.part * job.vecs) - gw * job.seg));
   };
 
-  // The copies run ahead: (pu, pc) is the next chunk to load.
-  long long pu = first;
-  int pc = 0;
-  float pw = weight_of(pu);
+  // The copies run ahead of the work by what the ring holds.
+  int done = 0;  // vectors of `ahead` that are loaded or on their way
+  int count = my_count(ahead);
+  float ahead_w = weight_of(ahead);
   auto load_next = [&] {
-    while (pu < units && (pw == 0.f || pc >= my_count(pu))) {
-      pu += stride;
-      pc = 0;
-      pw = weight_of(pu);
+    while (ahead.valid() && (ahead_w == 0.f || done >= count)) {
+      ahead.next();
+      done = 0;
+      count = my_count(ahead);
+      ahead_w = weight_of(ahead);
     }
-    if (pu >= units) return;
-    const int n = min(job.sub, my_count(pu) - pc);
-    ring.load(reinterpret_cast<const uint4*>(logits + (pu / job.parts) * job.ld) + my_first(pu) + pc, n * 16, lane);
-    pc += job.sub;
+    if (!ahead.valid()) return;
+    const int n = min(job.sub, count - done);
+    ring.load(reinterpret_cast<const uint4*>(logits + ahead.row * job.ld) + my_first(ahead) + done, n * 16, lane);
+    done += job.sub;
   };
   for (int i = 0; i < job.stages; ++i) load_next();
 
   bool ok = true;
   int k = 0;  // live units so far
-  float w = weight_of(first);
-  for (long long u = first; u < units; u += stride) {
-    const long long row = u / job.parts;
+  float w = weight_of(at);
+  for (; at.valid();) {
+    const UnitWalk u = at;
+    const long long row = u.row;
     const float weight = w;
-    w = weight_of(u + stride);
+    at.next();
+    w = weight_of(at);
     if (weight == 0.f) {
       if (kMode == kRowGrad) zero_vecs(dlogits + row * job.ld, job.ld / kV, gw * 32 + lane, G * 32);
       if (kMode != kRowStats && gw == 0 && lane == 0) policy_row_masked(args, row);
@@ -424,34 +498,29 @@ __global__ void __launch_bounds__(kRowThreads, 1) row_kernel(T* dlogits, const T
       ok = ok && ring.wait(4);
       const int nc = min(job.sub, n - c);
       if (!ok) break;
-      const uint4* x = ring.chunk();
       const int full = min(nc, job.V / kV - v0 - c);
-      int i = lane;
-      for (; i + 32 < full; i += 64) run.add<T>(x[i], x[i + 32]);
-      if (i < full) run.add<T>(x[i]);
-      if (full < nc && lane == 0) run.add<T>(cut_vec<T>(x[full], job.V % kV));
+      run.add_all<T>(ring.chunk(), full, full < nc, job.V % kV, lane);
       ring.step();
       if (kMode != kRowGrad) {
         __syncwarp();
         load_next();
       }
     }
-    const float m = warp_max_f(run.top);
-    const float s = warp_sum_f(run.s * exp_diff(run.m - finite_max(m)));
+    const RowSum sum = run.join();
     // Two sets of sums: a set is rewritten two rows on, and between lies a
     // meeting that the group's first warp reaches only after reading it.
-    if (lane == 0) sums[k & 1][warp] = make_float2(m, s);
+    if (lane == 0) sums[k & 1][warp] = sum;
     meet();
     if (gw == 0) {
-      const float2 p = lane < G ? sums[k & 1][warp + lane] : make_float2(-INFINITY, 0.f);
-      const float M = warp_max_f(p.x);
+      const RowSum p = lane < G ? sums[k & 1][warp + lane] : RowSum{0.0, -INFINITY};
+      const float M = warp_max_f(p.m);
       const float ref = finite_max(M);
-      const double S = warp_sum_d(static_cast<double>(p.y * expf(p.x - ref)));
+      const double S = warp_sum_d(p.s * exp(static_cast<double>(p.m - ref)));
       if (lane == 0) {
         if (kMode == kRowStats) {
-          job.slots[(u % job.parts) * job.rows + row] = make_float2(M, static_cast<float>(S));
+          job.slots[static_cast<long long>(u.part) * job.rows + row] = RowSum{S, M};
         } else {
-          const double c = policy_row(args, r, row, weight, static_cast<double>(xt) - static_cast<double>(M) - log_sum(S));
+          const double c = policy_row(args, r, row, weight, static_cast<double>(xt) - static_cast<double>(M) - log(S));
           if (kMode == kRowGrad) coef[warp] = RowCoef{ref, static_cast<float>(c / S), static_cast<float>(c), r.target};
         }
       }
@@ -471,7 +540,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) row_kernel(T* dlogits, const T
         }
       } else if (ok) {
         const RowGradient<T> g(rc);
-        float at = 0.f;
+        float value = 0.f;  // the gradient at the target
         bool target_here = false;
         for (int c = 0; c < n; c += job.sub) {
           const int nc = min(job.sub, n - c);
@@ -479,13 +548,13 @@ __global__ void __launch_bounds__(kRowThreads, 1) row_kernel(T* dlogits, const T
           const int t = rc.target - (v0 + c) * kV;
           if (t >= 0 && t < nc * kV && rc.target < job.V) {
             target_here = true;
-            at = g.at_target(elem_to_float(reinterpret_cast<const T*>(ring.chunk())[t]), rc.c);
+            value = g.at_target(elem_to_float(reinterpret_cast<const T*>(ring.chunk())[t]), rc.c);
           }
           ring.step();
           __syncwarp();
           load_next();
         }
-        if (target_here && lane == 0) elem_store(d + rc.target, at);
+        if (target_here && lane == 0) elem_store(d + rc.target, value);
       }
       if (gw == G - 1) zero_vecs(reinterpret_cast<uint4*>(d) + row_vecs, job.ld / kV - row_vecs, lane, 32);
     }
@@ -496,7 +565,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) row_kernel(T* dlogits, const T
 // The policy loss from slots, one thread a row (rows too long for row_kernel to
 // keep).
 template <typename T>
-__global__ void __launch_bounds__(128) policy_rows_kernel(RowCoef* __restrict__ coefs, const float2* __restrict__ slots,
+__global__ void __launch_bounds__(128) policy_rows_kernel(RowCoef* __restrict__ coefs, const RowSum* __restrict__ slots,
                                                           const T* __restrict__ logits, PolicyArgs a, int rows, int V,
                                                           int ld, int nslots) {
   const long long row = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
@@ -532,7 +601,7 @@ __device__ __forceinline__ double softplus_d(double v) { return (v > 0.0 ? v : 0
 constexpr int kPairThreads = 1024;
 template <typename T>
 __global__ void __launch_bounds__(kPairThreads) preference_pair_kernel(RowCoef* __restrict__ coefs,
-                                                                       float2* __restrict__ slots,
+                                                                       RowSum* __restrict__ slots,
                                                                        const T* __restrict__ logits, PreferenceArgs a,
                                                                        int pairs, int Tlen, int V, int ld, int nslots) {
   __shared__ double red[2][kPairThreads / 32];
@@ -618,30 +687,30 @@ __global__ void __launch_bounds__(kRowThreads, 1) row_gradient_kernel(T* dlogits
   WarpRing ring{smem + static_cast<size_t>(warp) * stages * sub * 16, bars + warp * kMaxStages, stages, sub * 16};
   ring.status = status;
   ring.abort_flag = &abort_word;
-  const int row_vecs = ld / kV, upr = (row_vecs + sub - 1) / sub;
-  const long long units = static_cast<long long>(rows) * upr;
-  const long long stride = static_cast<long long>(gridDim.x) * kRowWarps;
-  const long long first = static_cast<long long>(warp) * gridDim.x + blockIdx.x;
-  auto coef_of = [&](long long u) { return u < units ? coefs[u / upr] : RowCoef{0.f, 0.f, 0.f, -1}; };
-  auto first_vec = [&](long long u) { return static_cast<int>(u % upr) * sub; };
-  long long pu = first;
-  float pc = coef_of(pu).c;
+  const int row_vecs = ld / kV;
+  UnitWalk at(static_cast<long long>(warp) * gridDim.x + blockIdx.x, static_cast<long long>(gridDim.x) * kRowWarps, rows,
+              (row_vecs + sub - 1) / sub);
+  UnitWalk ahead = at;
+  auto coef_of = [&](const UnitWalk& u) { return u.valid() ? coefs[u.row] : RowCoef{0.f, 0.f, 0.f, -1}; };
+  float ahead_c = coef_of(ahead).c;
   auto load_next = [&] {
-    while (pu < units && pc == 0.f) pu += stride, pc = coef_of(pu).c;
-    if (pu >= units) return;
-    const int v0 = first_vec(pu);
-    ring.load(reinterpret_cast<const uint4*>(logits + (pu / upr) * ld) + v0, min(sub, row_vecs - v0) * 16, lane);
-    pu += stride;
-    pc = coef_of(pu).c;
+    while (ahead.valid() && ahead_c == 0.f) ahead.next(), ahead_c = coef_of(ahead).c;
+    if (!ahead.valid()) return;
+    const int v0 = ahead.part * sub;
+    ring.load(reinterpret_cast<const uint4*>(logits + ahead.row * ld) + v0, min(sub, row_vecs - v0) * 16, lane);
+    ahead.next();
+    ahead_c = coef_of(ahead).c;
   };
   for (int i = 0; i < stages; ++i) load_next();
   bool ok = true;
-  RowCoef next = coef_of(first);
-  for (long long u = first; u < units; u += stride) {
+  RowCoef next = coef_of(at);
+  while (at.valid()) {
+    const UnitWalk u = at;
     const RowCoef rc = next;
-    next = coef_of(u + stride);
-    const int v0 = first_vec(u), n = min(sub, row_vecs - v0);
-    T* d = dlogits + (u / upr) * ld;
+    at.next();
+    next = coef_of(at);
+    const int v0 = u.part * sub, n = min(sub, row_vecs - v0);
+    T* d = dlogits + u.row * ld;
     if (rc.c == 0.f) {
       zero_vecs(reinterpret_cast<uint4*>(d) + v0, n, lane, 32);
       continue;
@@ -674,7 +743,7 @@ int parts_of(long long rows, int V) {
 // Scratch of `rows` rows of `Vp` columns: the slot planes, then one RowCoef per
 // row.
 size_t slots_bytes(long long rows, int Vp) {
-  return (static_cast<size_t>(parts_of(rows, Vp)) * rows * sizeof(float2) + 15) / 16 * 16;
+  return static_cast<size_t>(parts_of(rows, Vp)) * rows * sizeof(RowSum);
 }
 size_t loss_workspace(long long rows, int Vp) { return slots_bytes(rows, Vp) + static_cast<size_t>(rows) * sizeof(RowCoef); }
 
@@ -759,7 +828,7 @@ RowJob row_job(const float* weights, int rows, int V, int Vp) {
 
 // Slots of every live row; returns the number of planes through *nslots.
 template <typename T>
-int launch_slots(float2* slots, int* nslots, const void* logits, const float* weights, int rows, int V, int Vp, cudaStream_t s) {
+int launch_slots(RowSum* slots, int* nslots, const void* logits, const float* weights, int rows, int V, int Vp, cudaStream_t s) {
   RowJob job = row_job<T>(weights, rows, V, Vp);
   const int all = job.vecs;
   job.slots = slots;
@@ -793,7 +862,7 @@ int policy_loss(void* dlogits, const void* logits, const PolicyArgs& a, int rows
     return launch_rows<T, kRowEval>(nullptr, logits, job, a, s);
   }
   if (share_out(&job, true)) return launch_rows<T, kRowGrad>(dlogits, logits, job, a, s);
-  auto* slots = static_cast<float2*>(workspace);
+  auto* slots = static_cast<RowSum*>(workspace);
   auto* coefs = reinterpret_cast<RowCoef*>(static_cast<char*>(workspace) + slots_bytes(rows, Vp));
   int nslots = 0;
   LLMK_TRY(launch_slots<T>(slots, &nslots, logits, a.weights, rows, V, Vp, s));
@@ -808,7 +877,7 @@ template <typename T>
 int preference_loss(void* dlogits, const void* logits, const PreferenceArgs& a, int pairs, int Tlen, int V, int Vp,
                     void* workspace, cudaStream_t s) {
   const int rows = 2 * pairs * Tlen;
-  auto* slots = static_cast<float2*>(workspace);
+  auto* slots = static_cast<RowSum*>(workspace);
   auto* coefs = dlogits ? reinterpret_cast<RowCoef*>(static_cast<char*>(workspace) + slots_bytes(rows, Vp)) : nullptr;
   int nslots = 0;
   LLMK_TRY(launch_slots<T>(slots, &nslots, logits, a.weights, rows, V, Vp, s));
