@@ -191,7 +191,7 @@ __device__ __forceinline__ float sum_exp_vec(const uint4& u, float ref, float* f
   float v[kV];
   unpack_vec(u, v);
 #pragma unroll
-  for (int j = 0; j < kV; ++j) v[j] = exp_diff(v[j] - ref);
+  for (int j = 0; j < kV; ++j) v[j] = ex2_approx((v[j] - ref) * kLog2e);
   *first = v[0];
 #pragma unroll
   for (int n = kV / 2; n > 0; n >>= 1)
@@ -207,13 +207,13 @@ __device__ __forceinline__ float first_elem(const uint4& u) {
 // A running maximum and the sum of exp(x - m), where m follows the largest
 // value seen, but only once that is more than 10 above it: the terms stay far
 // inside fp32's range, and a rescaling is rare.
-// ex2.approx is 5e-8 low on average, a little more or less by the spread of the
-// logits (measured), and a sum over a vocabulary keeps that mean while the
-// rounding errors cancel; a preference loss adds such sums over a thousand
-// positions. So one term in 16 is also computed by expf (6e-9 high on average),
-// and the sum is corrected by what those terms differ by: the mean error of a
-// row's log-probability falls from 5e-8 to 3e-9 for one more instruction per
-// element.
+// ex2.approx is 5e-8 low on average (measured), and one fp32 product by log2 e
+// moves a term by its distance times 1.3e-8. A sum over a vocabulary keeps the
+// mean of that while the rounding errors cancel, and a preference loss adds such
+// sums over a thousand positions. So one term in 16 is also computed by expf
+// (6e-9 high on average), and the sum is corrected by what those terms differ
+// by: the mean error of a row's log-probability falls from 5e-8 to below 1e-8
+// for one more instruction per element.
 struct RunningSum {
   float top = -INFINITY, m = -INFINITY, s = 0.f;
   float part = 0.f, off = 0.f;  // the terms computed twice: their sum, and what it lacks
@@ -393,7 +393,7 @@ struct UnitWalk {
 };
 
 enum RowMode { kRowGrad, kRowEval, kRowStats };
-constexpr int kRowWarps = 16;
+constexpr int kRowWarps = 24;
 constexpr int kRowThreads = 32 * kRowWarps;
 
 // How row_kernel shares rows out. A unit is a row (kRowStats: one of `parts`
@@ -778,26 +778,27 @@ int allow_smem(K kernel, size_t bytes, bool (&done)[64]) {
 
 int div_up(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
 
-// Bytes of shared memory that a warp's ring may take: 16 of them and the static
+// Bytes of shared memory that a warp's ring may take: all of them and the static
 // part fit the 227 KB of an SM.
-constexpr int kWarpRingBytes = 14336;
+constexpr int kWarpRingBytes = 9216;
 
 // Fills in group, seg, sub and stages for units of job.vecs vectors; false when
 // `keep` is asked (a unit stays in its group's rings) and it does not fit.
 bool share_out(RowJob* job, bool keep) {
   const int warp_vecs = kWarpRingBytes / 16;
   const long long units = static_cast<long long>(job->rows) * job->parts;
+  static const int kGroups[] = {1, 2, 3, 4, 6, 8, 12, 24};  // the divisors of kRowWarps
   // the fewest warps a unit fits, so that groups work on rows of their own and
   // one's barriers are hidden by the others, ...
-  int group = 1;
-  while (group < kRowWarps && job->vecs > group * warp_vecs) group *= 2;
-  if (keep && job->vecs > group * warp_vecs) return false;
+  int g = 0;
+  while (kGroups[g] < kRowWarps && job->vecs > kGroups[g] * warp_vecs) ++g;
+  if (keep && job->vecs > kGroups[g] * warp_vecs) return false;
   // ... but no fewer than it takes to keep all warps busy with few units
-  while (group < kRowWarps && units * group < static_cast<long long>(num_sms()) * kRowWarps && job->vecs > 32 * group) group *= 2;
-  job->group = group;
-  job->seg = div_up(job->vecs, group);
-  const int chunks = std::max(1, std::min(div_up(job->seg, 256), 4));
-  job->sub = std::min(div_up(div_up(job->seg, chunks), 32) * 32, 256);
+  while (kGroups[g] < kRowWarps && units * kGroups[g] < static_cast<long long>(num_sms()) * kRowWarps && job->vecs > 32 * kGroups[g]) ++g;
+  job->group = kGroups[g];
+  job->seg = div_up(job->vecs, job->group);
+  const int chunks = std::max(1, std::min(div_up(job->seg, 192), 3));
+  job->sub = std::min(div_up(div_up(job->seg, chunks), 32) * 32, 192);
   job->stages = std::min(kMaxStages, warp_vecs / job->sub);
   return !keep || job->stages * job->sub >= job->seg;
 }
@@ -842,7 +843,7 @@ template <typename T>
 int launch_gradient(void* dlogits, const void* logits, const RowCoef* coefs, int rows, int V, int Vp, cudaStream_t s) {
   static bool done[64] = {};
   LLMK_TRY(allow_smem(row_gradient_kernel<T>, kRowWarps * kWarpRingBytes, done));
-  const int vecs = Vp / vec_elems<T>(), chunks = div_up(vecs, 224), sub = div_up(div_up(vecs, chunks), 32) * 32;
+  const int vecs = Vp / vec_elems<T>(), chunks = div_up(vecs, 192), sub = div_up(div_up(vecs, chunks), 32) * 32;
   const int stages = std::min(kMaxStages, kWarpRingBytes / (sub * 16));
   const long long units = static_cast<long long>(rows) * div_up(vecs, sub);
   row_gradient_kernel<T><<<static_cast<int>(std::min<long long>(units, num_sms())), kRowThreads,
