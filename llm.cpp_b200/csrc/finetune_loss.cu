@@ -31,11 +31,12 @@ constexpr int vec_elems() {  // elements of a 16-byte vector
   return 16 / static_cast<int>(sizeof(T));
 }
 
-// The maximum of a row, or of part of one, and the sum of exp(x - max). The sum
-// is a double: what corrects it is less than half a step of fp32.
+// The maximum of a row, or of part of one, the sum of exp(x - max), and (whole
+// rows) the target's logit. The sum is a double: what corrects it is less than
+// half a step of fp32.
 struct __align__(16) RowSum {
   double s;
-  float m;
+  float m, xt;
 };
 
 // What the gradient of a row is made of.
@@ -136,6 +137,29 @@ __device__ __forceinline__ double policy_row(const PolicyArgs& a, const PolicyRo
   if (a.logps) a.logps[row] = static_cast<float>(lp);
   return g * w * a.dscale;
 }
+// The same coefficient in fp32, for the gradient: rho = exp(xt - max - old) / sum
+// and exp(d) = exp(ref - xt + max) sum need no logarithm, and two exponentials
+// side by side take a fourth of policy_row's time, which the row's warps would
+// wait for. Off by a few steps of fp32, as the exponentials it multiplies.
+__device__ __forceinline__ float policy_coef(const PolicyArgs& a, const PolicyRow& r, float w, const RowSum& t) {
+  auto exp_d = [](double v) {  // exp of a difference that one float does not hold
+    const float h = static_cast<float>(v);
+    return expf(h) * (1.f + (isfinite(h) ? static_cast<float>(v - static_cast<double>(h)) : 0.f));
+  };
+  const double x = static_cast<double>(t.xt) - static_cast<double>(t.m);
+  const float s = static_cast<float>(t.s);
+  const bool lost = isnan(x) || isnan(s);
+  float rho = 1.f;
+  if (a.old_logps) {
+    const double v = x - static_cast<double>(r.old);
+    rho = v > 80.0 ? exp_d(v - 64.0) * (6.2351491e27f / s) : exp_d(v) / s;  // e^64: a ratio that fp32 holds
+  }
+  const float clamped = fminf(fmaxf(rho, 1.f - a.clip_low), 1.f + a.clip_high);
+  const float s1 = r.adv == 0.f ? 0.f : rho * r.adv, s2 = clamped * r.adv;
+  float g = s1 > s2 ? 0.f : -s1;
+  if (a.kl_coef != 0.f) g -= a.kl_coef * (exp_d(static_cast<double>(r.ref) - x) * s - 1.f);
+  return lost ? NAN : g * w * a.dscale;
+}
 __device__ __forceinline__ void policy_row_masked(const PolicyArgs& a, long long row) {
   a.losses[row] = 0.f;
   if (a.kls) a.kls[row] = 0.f;
@@ -159,14 +183,20 @@ __device__ __forceinline__ void unpack_vec(const uint4& u, float (&v)[4]) {
   v[0] = __uint_as_float(u.x); v[1] = __uint_as_float(u.y); v[2] = __uint_as_float(u.z); v[3] = __uint_as_float(u.w);
 }
 template <typename T>
-__device__ __forceinline__ float max_vec(const uint4& u) {
+__device__ __forceinline__ float max_vec(const uint4& u, const uint4& w) {
   if constexpr (sizeof(T) == 2) {
     auto h = [](const uint32_t& v) { return *reinterpret_cast<const __nv_bfloat162*>(&v); };
-    const __nv_bfloat162 m = __hmax2(__hmax2(h(u.x), h(u.y)), __hmax2(h(u.z), h(u.w)));
+    const __nv_bfloat162 m = __hmax2(__hmax2(__hmax2(h(u.x), h(u.y)), __hmax2(h(u.z), h(u.w))),
+                                     __hmax2(__hmax2(h(w.x), h(w.y)), __hmax2(h(w.z), h(w.w))));
     return fmaxf(__low2float(m), __high2float(m));
   } else {
-    return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+    auto f = [](uint32_t v) { return __uint_as_float(v); };
+    return fmaxf(fmaxf(fmaxf(f(u.x), f(u.y)), fmaxf(f(u.z), f(u.w))), fmaxf(fmaxf(f(w.x), f(w.y)), fmaxf(f(w.z), f(w.w))));
   }
+}
+template <typename T>
+__device__ __forceinline__ float max_vec(const uint4& u) {
+  return max_vec<T>(u, u);
 }
 // The elements from `keep` on replaced by -inf.
 template <typename T>
@@ -204,23 +234,29 @@ __device__ __forceinline__ float first_elem(const uint4& u) {
   return __uint_as_float(sizeof(T) == 2 ? u.x << 16 : u.x);
 }
 
-// A running maximum and the sum of exp(x - m), where m follows the largest
-// value seen, but only once that is more than 10 above it: the terms stay far
-// inside fp32's range, and a rescaling is rare.
+// A warp's running maximum and sum of exp(x - m). m starts as the maximum over
+// the warp's first vectors and, in a lane, follows a value more than 10 above it:
+// the terms stay far inside fp32's range, and a lane that raises m is rare.
 // ex2.approx is 5e-8 low on average (measured), and one fp32 product by log2 e
 // moves a term by its distance times 1.3e-8. A sum over a vocabulary keeps the
 // mean of that while the rounding errors cancel, and a preference loss adds such
-// sums over a thousand positions. So one term in 16 is also computed by expf
-// (6e-9 high on average), and the sum is corrected by what those terms differ
-// by: the mean error of a row's log-probability falls from 5e-8 to below 1e-8
-// for one more instruction per element.
+// sums over a thousand positions. So one term in 16 is also computed by expf, and
+// the sum is corrected by what those terms differ by: the mean error of a row's
+// log-probability falls from 5e-8 to below 1e-8 for one more instruction per
+// element.
+struct __align__(8) WarpSum {
+  float top, m, s;
+  float part, off;  // the terms computed twice: their sum, and what it lacks
+  float unused;
+};
 struct RunningSum {
-  float top = -INFINITY, m = -INFINITY, s = 0.f;
-  float part = 0.f, off = 0.f;  // the terms computed twice: their sum, and what it lacks
+  float top = -INFINITY, m = -INFINITY, m0 = -INFINITY, s = 0.f;
+  float part = 0.f, off = 0.f;
+  __device__ __forceinline__ void start(float vm) { m = m0 = warp_max_f(vm); }
   __device__ __forceinline__ float raise(float vm) {
     top = fmaxf(top, vm);
     if (!(vm <= m + 10.f)) {
-      const float f = ex2_approx((m - vm) * kLog2e);
+      const float f = expf(m - vm);
       s *= f, part *= f, off *= f;
       m = vm;
     }
@@ -239,7 +275,7 @@ struct RunningSum {
   }
   template <typename T>
   __device__ __forceinline__ void add(const uint4& u, const uint4& w) {
-    const float ref = raise(fmaxf(max_vec<T>(u), max_vec<T>(w)));
+    const float ref = raise(max_vec<T>(u, w));
     float e, unused;
     s += sum_exp_vec<T>(u, ref, &e) + sum_exp_vec<T>(w, ref, &unused);
     if (sizeof(T) == 2) twice(first_elem<T>(u), ref, e);
@@ -247,7 +283,7 @@ struct RunningSum {
   // fp32 vectors are half as long
   template <typename T>
   __device__ __forceinline__ void add(const uint4& a, const uint4& b, const uint4& c, const uint4& d) {
-    const float ref = raise(fmaxf(fmaxf(max_vec<T>(a), max_vec<T>(b)), fmaxf(max_vec<T>(c), max_vec<T>(d))));
+    const float ref = raise(fmaxf(max_vec<T>(a, b), max_vec<T>(c, d)));
     float e, unused;
     s += (sum_exp_vec<T>(a, ref, &e) + sum_exp_vec<T>(b, ref, &unused)) +
          (sum_exp_vec<T>(c, ref, &unused) + sum_exp_vec<T>(d, ref, &unused));
@@ -263,40 +299,60 @@ struct RunningSum {
     if (i < full) add<T>(x[i]);
     if (partial && lane == 0) add<T>(cut_vec<T>(x[full], keep));
   }
-  // The warp's maximum and sum of exp(x - maximum); the maximum's own term is
-  // exactly 1 and needs no correction.
-  __device__ __forceinline__ RowSum join() const {
-    const float M = warp_max_f(top);
-    // one factor for all of the lane's terms: expf's error would not cancel
-    const double f = exp(static_cast<double>(m - finite_max(M)));
-    const double S = warp_sum_d(static_cast<double>(s) * f);
-    const float P = warp_sum_f(part * static_cast<float>(f)), D = warp_sum_f(off * static_cast<float>(f));
-    return RowSum{P > 0.f ? S + (S - 1.0) * (static_cast<double>(D / P) - 6e-9) : S, M};
+  // The warp's sums, at one m.
+  __device__ __forceinline__ WarpSum join() const {
+    WarpSum w{warp_max_f(top), m0, s, part, off, 0.f};
+    if (__any_sync(0xffffffffu, m != m0)) {  // also where m is NaN
+      w.m = warp_max_f(m);
+      const float f = expf(m - finite_max(w.m));
+      w.s *= f, w.part *= f, w.off *= f;
+    }
+    w.s = warp_sum_f(w.s), w.part = warp_sum_f(w.part), w.off = warp_sum_f(w.off);
+    return w;
   }
 };
+
+// A row's sum from its warps' (lanes >= count: none), the same in every lane.
+__device__ __forceinline__ RowSum fold_warps(const WarpSum* sums, int count, int lane) {
+  WarpSum w{-INFINITY, -INFINITY, 0.f, 0.f, 0.f, 0.f};
+  if (lane < count) w = sums[lane];
+  const float M = warp_max_f(w.top);
+  const float f = expf(w.m - finite_max(M));
+  const float S = warp_sum_f(w.s * f), P = warp_sum_f(w.part * f), D = warp_sum_f(w.off * f);
+  // expf itself is 6e-9 high on average, in the terms and in the factors; the
+  // maximum's own term is 1 and needs no correction
+  const double s = S;
+  return RowSum{P > 0.f ? s + (s - 1.0) * (static_cast<double>(D / P) - 1.2e-8) : s, M, 0.f};
+}
 
 // -exp(x - max) scale over a vector: the gradient everywhere but at the target.
 template <typename T>
 struct RowGradient {
   float max, scale;
-  float k;        // 16-bit output: log2 |scale|, folded into the exponent,
-  uint32_t flip;  // and its sign
-  __device__ __forceinline__ explicit RowGradient(const RowCoef& c) : max(c.max), scale(c.scale), k(0.f), flip(0) {
-    if constexpr (sizeof(T) == 2) {
-      k = log2f(fabsf(scale));
-      flip = scale > 0.f ? 0x80008000u : 0u;
-    }
+  float k;  // 16-bit output: log2 |scale|, folded into the exponent
+  __device__ __forceinline__ explicit RowGradient(const RowCoef& c) : max(c.max), scale(c.scale), k(0.f) {
+    if constexpr (sizeof(T) == 2) k = log2f(fabsf(scale));
   }
+  // kMode, 16-bit output: 0 any row; 1 and 2 rows of |max| < 512 and of positive
+  // or negative scale, where x log2 e - max log2 e in one rounding is off by at
+  // most 2^-14 relative, far inside the 2^-8 the result is rounded by.
+  template <int kMode>
   __device__ __forceinline__ uint4 of(const uint4& u) const {
     constexpr int kV = vec_elems<T>();
     float v[kV];
     unpack_vec(u, v);
     if constexpr (sizeof(T) == 2) {
-      // rounded to bf16 anyway: one product by log2 e is exact enough
+      const float c = fmaf(-max, kLog2e, k);
       uint32_t w[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        w[i] = pack_bf16x2(ex2_approx(fmaf(v[2 * i] - max, kLog2e, k)), ex2_approx(fmaf(v[2 * i + 1] - max, kLog2e, k))) ^ flip;
+      for (int i = 0; i < 4; ++i) {
+        float a[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          a[j] = ex2_approx(kMode ? fmaf(v[2 * i + j], kLog2e, c) : fmaf(v[2 * i + j] - max, kLog2e, k));
+        if (kMode == 2 || (kMode == 0 && !(scale > 0.f))) w[i] = pack_bf16x2(a[0], a[1]);
+        else w[i] = pack_bf16x2(-a[0], -a[1]);
+      }
       return make_uint4(w[0], w[1], w[2], w[3]);
     } else {
 #pragma unroll
@@ -304,20 +360,29 @@ struct RowGradient {
       return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
     }
   }
+  template <int kMode>
+  __device__ __forceinline__ void store_full(uint4* d, const uint4* x, int full, int lane) const {
+    int i = lane;
+    for (; i + 32 < full; i += 64) {
+      const uint4 a = x[i], b = x[i + 32];
+      d[i] = of<kMode>(a);
+      d[i + 32] = of<kMode>(b);
+    }
+    if (i < full) d[i] = of<kMode>(x[i]);
+  }
   // `n` vectors of a row, the first of them number v0, by one warp; the row's
   // last, partly live vector gets zeros in its padding.
   __device__ __forceinline__ void store(T* row, const uint4* x, int v0, int n, int V, int lane) const {
     uint4* d = reinterpret_cast<uint4*>(row) + v0;
     const int full = min(n, V / vec_elems<T>() - v0);
-    int i = lane;
-    for (; i + 32 < full; i += 64) {
-      const uint4 a = x[i], b = x[i + 32];
-      d[i] = of(a);
-      d[i + 32] = of(b);
+    if (sizeof(T) == 2 && fabsf(max) < 512.f) {
+      if (scale > 0.f) store_full<1>(d, x, full, lane);
+      else store_full<2>(d, x, full, lane);
+    } else {
+      store_full<0>(d, x, full, lane);
     }
-    if (i < full) d[i] = of(x[i]);
     if (full < n && lane == 0) {
-      const uint4 o = of(x[full]);
+      const uint4 o = of<0>(x[full]);
       uint32_t w[4] = {o.x, o.y, o.z, o.w};
       const int keep = V % vec_elems<T>();
 #pragma unroll
@@ -400,7 +465,7 @@ constexpr int kRowThreads = 32 * kRowWarps;
 // parts of it) of `vecs` vectors; `group` warps take a unit, each `seg` vectors
 // of it, through its ring in chunks of `sub`.
 struct RowJob {
-  RowSum* slots;  // kRowStats
+  RowSum* slots;
   const float* weights;
   int rows, V, ld;
   int parts, vecs, group, seg, sub, stages;
@@ -409,19 +474,19 @@ struct RowJob {
 
 // One pass over the rows, one persistent CTA of 16 warps per SM. Groups of
 // warps take one row each: pass A waits for the warp's chunks as they arrive and
-// folds them into its running sum; the group's sums are joined, and its first
-// thread does the row's scalar work in 64 bits; in kRowGrad the chunks stay in
+// folds them into its running sum; the group's first warp joins the sums and
+// forms the row's coefficient; in kRowGrad the chunks stay in
 // shared memory until pass B has written the gradient from them, so the logits
 // are read from memory once, and each chunk's place is then refilled with the
-// group's next row. Masked rows take no chunk. kRowStats leaves (max, sum) of
-// each unit in its slot, planes of `rows`. A wait that is given up (the device
+// group's next row. Masked rows take no chunk. Each unit's (max, sum) goes to its
+// slot, planes of `rows`. A wait that is given up (the device
 // status says so) ends the work, not the barriers: the group's warps still meet.
 template <typename T, int kMode>
 __global__ void __launch_bounds__(kRowThreads, 1) row_kernel(T* dlogits, const T* logits, RowJob job, PolicyArgs args) {
   constexpr int kV = vec_elems<T>();
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t bars[kRowWarps * kMaxStages];
-  __shared__ RowSum sums[2][kRowWarps];
+  __shared__ WarpSum sums[2][kRowWarps];
   __shared__ RowCoef coef[kRowWarps];
   __shared__ int abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -481,7 +546,6 @@ __global__ void __launch_bounds__(kRowThreads, 1) row_kernel(T* dlogits, const T
     w = weight_of(at);
     if (weight == 0.f) {
       if (kMode == kRowGrad) zero_vecs(dlogits + row * job.ld, job.ld / kV, gw * 32 + lane, G * 32);
-      if (kMode != kRowStats && gw == 0 && lane == 0) policy_row_masked(args, row);
       continue;
     }
     const int v0 = my_first(u), n = my_count(u);
@@ -498,30 +562,29 @@ __global__ void __launch_bounds__(kRowThreads, 1) row_kernel(T* dlogits, const T
       ok = ok && ring.wait(4);
       const int nc = min(job.sub, n - c);
       if (!ok) break;
+      const uint4* x = ring.chunk();
       const int full = min(nc, job.V / kV - v0 - c);
-      run.add_all<T>(ring.chunk(), full, full < nc, job.V % kV, lane);
+      if (c == 0) run.start(lane < full ? max_vec<T>(x[lane]) : -INFINITY);
+      run.add_all<T>(x, full, full < nc, job.V % kV, lane);
       ring.step();
       if (kMode != kRowGrad) {
         __syncwarp();
         load_next();
       }
     }
-    const RowSum sum = run.join();
+    const WarpSum sum = run.join();
     // Two sets of sums: a set is rewritten two rows on, and between lies a
     // meeting that the group's first warp reaches only after reading it.
     if (lane == 0) sums[k & 1][warp] = sum;
     meet();
     if (gw == 0) {
-      const RowSum p = lane < G ? sums[k & 1][warp + lane] : RowSum{0.0, -INFINITY};
-      const float M = warp_max_f(p.m);
-      const float ref = finite_max(M);
-      const double S = warp_sum_d(p.s * exp(static_cast<double>(p.m - ref)));
+      RowSum t = fold_warps(&sums[k & 1][warp], G, lane);
+      t.xt = xt;
       if (lane == 0) {
-        if (kMode == kRowStats) {
-          job.slots[static_cast<long long>(u.part) * job.rows + row] = RowSum{S, M};
-        } else {
-          const double c = policy_row(args, r, row, weight, static_cast<double>(xt) - static_cast<double>(M) - log(S));
-          if (kMode == kRowGrad) coef[warp] = RowCoef{ref, static_cast<float>(c / S), static_cast<float>(c), r.target};
+        job.slots[static_cast<long long>(u.part) * job.rows + row] = t;
+        if (kMode == kRowGrad) {
+          const float c = policy_coef(args, r, weight, t);
+          coef[warp] = RowCoef{finite_max(t.m), c / static_cast<float>(t.s), c, r.target};
         }
       }
     }
@@ -560,6 +623,20 @@ __global__ void __launch_bounds__(kRowThreads, 1) row_kernel(T* dlogits, const T
     }
   }
   ring.drain();
+  if (kMode == kRowStats) return;
+  // The losses of this CTA's rows, in 64 bits, a row a thread: beside the passes
+  // they would hold up a group for 2000 cycles a row.
+  __syncthreads();
+  for (long long row = blockIdx.x + static_cast<long long>(threadIdx.x) * gridDim.x; row < job.rows;
+       row += static_cast<long long>(kRowThreads) * gridDim.x) {
+    const float weight = job.weights ? job.weights[row] : 1.f;
+    if (weight == 0.f) {
+      policy_row_masked(args, row);
+    } else {
+      const RowSum t = job.slots[row];
+      policy_row(args, policy_row_load(args, row), row, weight, static_cast<double>(t.xt) - static_cast<double>(t.m) - log(t.s));
+    }
+  }
 }
 
 // The policy loss from slots, one thread a row (rows too long for row_kernel to
@@ -858,12 +935,13 @@ template <typename T>
 int policy_loss(void* dlogits, const void* logits, const PolicyArgs& a, int rows, int V, int Vp, void* workspace,
                 cudaStream_t s) {
   RowJob job = row_job<T>(a.weights, rows, V, Vp);
+  job.slots = static_cast<RowSum*>(workspace);
   if (!dlogits) {
     share_out(&job, false);
     return launch_rows<T, kRowEval>(nullptr, logits, job, a, s);
   }
   if (share_out(&job, true)) return launch_rows<T, kRowGrad>(dlogits, logits, job, a, s);
-  auto* slots = static_cast<RowSum*>(workspace);
+  RowSum* slots = job.slots;
   auto* coefs = reinterpret_cast<RowCoef*>(static_cast<char*>(workspace) + slots_bytes(rows, Vp));
   int nslots = 0;
   LLMK_TRY(launch_slots<T>(slots, &nslots, logits, a.weights, rows, V, Vp, s));
