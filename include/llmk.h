@@ -319,6 +319,26 @@ int llmk_preference_loss(float* losses, float* rewards, float* logps, void* dlog
                          llmk_dtype dtype, const int* targets, const float* weights, const float* ref_logps, int pairs,
                          int T, int V, int Vp, float beta, float label_smoothing, float dscale, void* workspace,
                          size_t workspace_bytes, void* stream);
+/* The two losses on top of the lm_head, as llmk_matmul_crossentropy_forward is
+ * the cross-entropy's: logits[BT, Vp] = inp[BT, C] * W[Vp, C]^T (+ bias) on the
+ * tensor cores, whose epilogue leaves each row's softmax statistics, so that the
+ * logits are not read to find the losses; with backward != 0 one more pass
+ * overwrites them with the gradient (0 in rows of weight 0). Arguments, outputs
+ * and refusals as above; BT = 2 * pairs * T for the preference loss. The
+ * statistics are those of the stored logits: with bf16 logits the
+ * log-probabilities carry their rounding. workspace >=
+ * llmk_matmul_finetune_workspace(BT, Vp). */
+size_t llmk_matmul_finetune_workspace(int BT, int Vp);
+int llmk_matmul_policy_forward(float* losses, float* kls, float* logps, void* logits, llmk_dtype dtype, const void* inp,
+                               const void* W, const float* bias, const int* targets, const float* weights,
+                               const float* advantages, const float* old_logps, const float* ref_logps, int BT, int C,
+                               int Vp, int V, float clip_low, float clip_high, float kl_coef, float dscale, int backward,
+                               llmk_math math, void* workspace, size_t workspace_bytes, void* stream);
+int llmk_matmul_preference_forward(float* losses, float* rewards, float* logps, void* logits, llmk_dtype dtype,
+                                   const void* inp, const void* W, const float* bias, const int* targets,
+                                   const float* weights, const float* ref_logps, int pairs, int T, int C, int Vp, int V,
+                                   float beta, float label_smoothing, float dscale, int backward, llmk_math math,
+                                   void* workspace, size_t workspace_bytes, void* stream);
 /* *out = mean(x[0..n)) on the device, fixed reduction order. */
 int llmk_mean(float* out, const float* x, int n, void* stream);
 

@@ -102,6 +102,35 @@ int llmk_gpt2_set_train_data(llmk_gpt2* model, const int* host_inputs, const int
  * leaves dlogits ready for llmk_gpt2_backward.
  * Replaces GPT2::Forward (gpt2cuda.cu:338-345). */
 int llmk_gpt2_forward(llmk_gpt2* model, const int* d_inputs, const int* d_targets);
+/* ------------------------------------------------ fine-tuning (new) */
+/* Log-probabilities of the targets at every position (d_logps: B*T floats in
+ * device memory), no gradient: what the losses below call old_logps (this model
+ * when it sampled) and ref_logps (a reference model). Asynchronous. */
+int llmk_gpt2_logprobs(llmk_gpt2* model, const int* d_inputs, const int* d_targets, float* d_logps);
+/* Forward with the clipped policy loss (llmk_policy_loss, whose arguments these
+ * are: device arrays of B*T floats, weights and old_logps optional, ref_logps
+ * needed with kl_coef or kls) in the place of the cross-entropy; leaves its
+ * gradient for llmk_gpt2_backward. The loss (llmk_gpt2_loss) is the sum over all
+ * positions: weights carry the normalisation. */
+int llmk_gpt2_forward_policy(llmk_gpt2* model, const int* d_inputs, const int* d_targets, const float* weights,
+                             const float* advantages, const float* old_logps, const float* ref_logps, float clip_low,
+                             float clip_high, float kl_coef, float* kls, float* logps);
+/* Forward with the preference loss (llmk_preference_loss) over B / 2 pairs:
+ * sequence p is the preferred one of pair p, sequence B/2 + p the other (B even).
+ * weights: B*T floats or NULL; ref_logps: B floats (sums over the sequences) or
+ * NULL; rewards: B floats or NULL; logps: B*T floats or NULL. The loss is the
+ * mean over the pairs. */
+int llmk_gpt2_forward_preference(llmk_gpt2* model, const int* d_inputs, const int* d_targets, const float* weights,
+                                 const float* ref_logps, float beta, float label_smoothing, float* rewards,
+                                 float* logps);
+/* Clips the global norm of the gradients (averaged over ranks) to max_norm in
+ * every later update, the captured ones included; 0 turns it off. The norm costs
+ * one pass over the gradients; AdamW scales them on the way in. Under data
+ * parallelism the update then starts once every bucket is reduced. */
+int llmk_gpt2_set_grad_clip(llmk_gpt2* model, float max_norm);
+/* Norm of the last clipped update's gradients before clipping (0 before the
+ * first). Synchronises the model stream. */
+int llmk_gpt2_grad_norm(llmk_gpt2* model, float* host_norm);
 /* Zeroes the gradients the backward accumulates into (GPT2::ZeroGrad, gpt2cuda.cu:548). */
 int llmk_gpt2_zero_grad(llmk_gpt2* model);
 /* Backward of the last forward; with data parallelism enabled, also the

@@ -88,13 +88,6 @@ __device__ __forceinline__ double target_logp(const T* logits, long long row, in
   return static_cast<double>(elem_to_float(logits[row * ld + target])) - static_cast<double>(m) - log(s);
 }
 
-struct PolicyArgs {
-  float *losses, *kls, *logps;
-  const int* targets;
-  const float *weights, *advantages, *old_logps, *ref_logps;
-  float clip_low, clip_high, kl_coef, dscale;
-};
-
 // The policy loss of one live row, given lp: writes the row's outputs and
 // returns d(loss)/d(lp) with weight and dscale. With rho = exp(lp - old), A the
 // advantage and d = ref - lp: loss = w (-min(rho A, clamp(rho) A) + kl_coef
@@ -165,10 +158,6 @@ __device__ __forceinline__ void policy_row_masked(const PolicyArgs& a, long long
   if (a.kls) a.kls[row] = 0.f;
   if (a.logps) a.logps[row] = 0.f;
 }
-
-// exp(d) for a difference d of logits: 2^(d log2 e) with the constant in two
-// parts, so that the product's error does not lean one way.
-__device__ __forceinline__ float exp_diff(float d) { return ex2_approx(fmaf(d, 1.44269502f, d * 1.92596299e-8f)); }
 
 // One 16-byte vector.
 __device__ __forceinline__ void unpack_vec(const uint4& u, float (&v)[8]) {
@@ -380,8 +369,13 @@ struct RowGradient {
       }
       return make_uint4(w[0], w[1], w[2], w[3]);
     } else {
+      const uint64_t m = f2_pack(-max, -max), l = f2_pack(kLog2e, kLog2e), sc = f2_pack(-scale, -scale);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = -exp_diff(v[j] - max) * scale;
+      for (int j = 0; j < 4; j += 2) {
+        float a, b;
+        f2_unpack(f2_mul(f2_add(f2_pack(v[j], v[j + 1]), m), l), a, b);
+        f2_unpack(f2_mul(f2_pack(ex2_approx(a), ex2_approx(b)), sc), v[j], v[j + 1]);
+      }
       return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
     }
   }
@@ -546,6 +540,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) row_kernel(T* dlogits, const T
   __shared__ RowList todo;
   __shared__ int abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (kMode == kRowStats) grid_release();
   const int first_row = job.row0 + blockIdx.x;
   const int n_items = (job.row1 - first_row + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
   auto row_of = [&](int item) { return first_row + static_cast<long long>(item) * gridDim.x; };
@@ -708,6 +703,8 @@ template <typename T>
 __global__ void __launch_bounds__(128) policy_rows_kernel(RowCoef* __restrict__ coefs, const RowSum* __restrict__ slots,
                                                           const T* __restrict__ logits, PolicyArgs a, int rows, int V,
                                                           int ld, int nslots) {
+  grid_release();
+  grid_wait();
   const long long row = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
   if (row >= rows) return;
   const float w = a.weights ? a.weights[row] : 1.f;
@@ -724,13 +721,6 @@ __global__ void __launch_bounds__(128) policy_rows_kernel(RowCoef* __restrict__ 
   if (coefs) coefs[row] = RowCoef{finite_max(m), static_cast<float>(c / s), static_cast<float>(c), r.target};
 }
 
-struct PreferenceArgs {
-  float *losses, *rewards, *logps;
-  const int* targets;
-  const float *weights, *ref_logps;
-  float beta, smoothing, dscale;
-};
-
 // log(1 + exp(v)) without overflow.
 __device__ __forceinline__ double softplus_d(double v) { return (v > 0.0 ? v : 0.0) + log1p(exp(-fabs(v))); }
 
@@ -745,6 +735,8 @@ __global__ void __launch_bounds__(kPairThreads) preference_pair_kernel(RowCoef* 
                                                                        const T* __restrict__ logits, PreferenceArgs a,
                                                                        int pairs, int Tlen, int V, int ld, int nslots) {
   __shared__ double red[2][kPairThreads / 32];
+  grid_release();
+  grid_wait();
   const int pair = blockIdx.x, rows = 2 * pairs * Tlen;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   double sum[2] = {0.0, 0.0};
@@ -827,6 +819,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) row_gradient_kernel(T* dlogits
     fence_mbar_init();
   }
   __syncthreads();
+  grid_wait();
   WarpRing ring{smem + static_cast<size_t>(warp) * stages * sub * 16, bars + warp * kMaxStages, stages, sub * 16};
   ring.status = status;
   ring.abort_flag = &abort_word;
@@ -1008,11 +1001,10 @@ int launch_gradient(void* dlogits, const void* logits, const RowCoef* coefs, int
   const int vecs = Vp / vec_elems<T>(), chunks = div_up(vecs, 192), sub = div_up(div_up(vecs, chunks), 32) * 32;
   const int stages = std::min(kMaxStages, kWarpRingBytes / (sub * 16));
   const long long units = static_cast<long long>(rows) * div_up(vecs, sub);
-  row_gradient_kernel<T><<<static_cast<int>(std::min<long long>(units, num_sms())), kRowThreads,
-                           static_cast<size_t>(kRowWarps) * stages * sub * 16, s>>>(
-      static_cast<T*>(dlogits), static_cast<const T*>(logits), coefs, rows, V, Vp, sub, stages, device_status_ptr());
+  LLMK_CUDA(launch_after(row_gradient_kernel<T>, static_cast<int>(std::min<long long>(units, num_sms())), kRowThreads,
+                         static_cast<size_t>(kRowWarps) * stages * sub * 16, s, static_cast<T*>(dlogits),
+                         static_cast<const T*>(logits), coefs, rows, V, Vp, sub, stages, device_status_ptr()));
   count_launch();
-  LLMK_CUDA(cudaGetLastError());
   return LLMK_OK;
 }
 
@@ -1030,10 +1022,9 @@ int policy_loss(void* dlogits, const void* logits, const PolicyArgs& a, int rows
   auto* coefs = dlogits ? reinterpret_cast<RowCoef*>(static_cast<char*>(workspace) + slots_bytes(rows, Vp)) : nullptr;
   int nslots = 0;
   LLMK_TRY(launch_slots<T>(slots, &nslots, logits, a.weights, rows, V, Vp, s));
-  policy_rows_kernel<T><<<div_up(rows, 128), 128, 0, s>>>(coefs, slots, static_cast<const T*>(logits), a, rows, V, Vp,
-                                                          nslots);
+  LLMK_CUDA(launch_after(policy_rows_kernel<T>, div_up(rows, 128), 128, 0, s, coefs, slots,
+                         static_cast<const T*>(logits), a, rows, V, Vp, nslots));
   count_launch();
-  LLMK_CUDA(cudaGetLastError());
   return dlogits ? launch_gradient<T>(dlogits, logits, coefs, rows, V, Vp, s) : LLMK_OK;
 }
 
@@ -1045,16 +1036,164 @@ int preference_loss(void* dlogits, const void* logits, const PreferenceArgs& a, 
   auto* coefs = dlogits ? reinterpret_cast<RowCoef*>(static_cast<char*>(workspace) + slots_bytes(rows, Vp)) : nullptr;
   int nslots = 0;
   LLMK_TRY(launch_slots<T>(slots, &nslots, logits, a.weights, rows, V, Vp, s));
-  preference_pair_kernel<T><<<pairs, kPairThreads, 0, s>>>(coefs, slots, static_cast<const T*>(logits), a, pairs, Tlen, V,
-                                                           Vp, nslots);
+  LLMK_CUDA(launch_after(preference_pair_kernel<T>, pairs, kPairThreads, 0, s, coefs, slots,
+                         static_cast<const T*>(logits), a, pairs, Tlen, V, Vp, nslots));
   count_launch();
-  LLMK_CUDA(cudaGetLastError());
   return dlogits ? launch_gradient<T>(dlogits, logits, coefs, rows, V, Vp, s) : LLMK_OK;
 }
 
 bool bad_nonneg(float v) { return !(v >= 0.f) || std::isinf(v); }
 
+// From the lm_head GEMM's statistics, (max, sum exp(x - max)) of every 64 columns
+// in planes of `rows`: block = 8 rows, 32 threads a row fold a 32nd of the slots
+// each, and one joins them in a fixed order.
+constexpr int kFoldRows = 8, kFoldGroups = 32;
+template <typename T>
+__global__ void __launch_bounds__(kFoldRows* kFoldGroups) rowstats_fold_kernel(RowSum* __restrict__ sums,
+                                                                              const float2* __restrict__ stats,
+                                                                              const T* __restrict__ logits,
+                                                                              const int* __restrict__ targets, int rows,
+                                                                              int V, int ld, int nslots) {
+  __shared__ float2 part[kFoldGroups][kFoldRows];
+  grid_release();
+  grid_wait();
+  const int r = threadIdx.x % kFoldRows, g = threadIdx.x / kFoldRows;
+  const long long row = static_cast<long long>(blockIdx.x) * kFoldRows + r;
+  float m = -INFINITY, s = 0.f;
+  if (row < rows) {
+    for (int k = g; k < nslots; k += kFoldGroups) {
+      const float2 p = stats[static_cast<long long>(k) * rows + row];
+      const float top = fmaxf(m, p.x), ref = finite_max(top);
+      s = s * expf(m - ref) + p.y * expf(p.x - ref);
+      m = top;
+    }
+  }
+  part[g][r] = make_float2(m, s);
+  __syncthreads();
+  if (g != 0 || row >= rows) return;
+  float M = -INFINITY;
+  for (int i = 0; i < kFoldGroups; ++i) M = fmaxf(M, part[i][r].x);
+  double S = 0.0;
+  for (int i = 0; i < kFoldGroups; ++i) S += static_cast<double>(part[i][r].y) * static_cast<double>(expf(part[i][r].x - finite_max(M)));
+  const int t = targets[row];
+  sums[row] = RowSum{S, M, t >= 0 && t < V ? elem_to_float(logits[row * ld + t]) : NAN};
+}
+
+__global__ void __launch_bounds__(256) logps_kernel(float* __restrict__ logps, const RowSum* __restrict__ sums, int rows) {
+  grid_wait();
+  const long long row = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (row >= rows) return;
+  const RowSum t = sums[row];
+  logps[row] = static_cast<float>(static_cast<double>(t.xt) - static_cast<double>(t.m) - log(t.s));
+}
+
+__global__ void __launch_bounds__(1024) sum_losses_kernel(float* __restrict__ out, const float* __restrict__ x, int n, float div) {
+  __shared__ double red[32];
+  double s = 0.0;
+  for (int i = threadIdx.x; i < n; i += 1024) s += x[i];
+  s = warp_sum_d(s);
+  if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = s;
+  __syncthreads();
+  if (threadIdx.x >= 32) return;
+  s = warp_sum_d(red[threadIdx.x]);
+  if (threadIdx.x == 0) *out = static_cast<float>(s / div);
+}
+
+template <typename T>
+int launch_fold(RowSum* sums, const float2* stats, const void* logits, const int* targets, int rows, int V, int ld, cudaStream_t s) {
+  LLMK_CUDA(launch_after(rowstats_fold_kernel<T>, div_up(rows, kFoldRows), kFoldRows * kFoldGroups, 0, s, sums, stats,
+                         static_cast<const T*>(logits), targets, rows, V, ld, div_up(ld, 64)));
+  count_launch();
+  return LLMK_OK;
+}
+
+struct Scratch {
+  RowSum* sums;
+  RowCoef* coefs;
+};
+Scratch split(void* scratch, int rows) {
+  auto* sums = static_cast<RowSum*>(scratch);
+  return {sums, reinterpret_cast<RowCoef*>(sums + rows)};
+}
+
+template <typename T>
+int policy_finish_t(void* logits, const float2* stats, const PolicyArgs& a, int rows, int V, int ld, int backward,
+                    void* scratch, cudaStream_t s) {
+  const Scratch w = split(scratch, rows);
+  LLMK_TRY(launch_fold<T>(w.sums, stats, logits, a.targets, rows, V, ld, s));
+  RowCoef* coefs = backward ? w.coefs : nullptr;
+  LLMK_CUDA(launch_after(policy_rows_kernel<T>, div_up(rows, 128), 128, 0, s, coefs, w.sums,
+                         static_cast<const T*>(logits), a, rows, V, ld, 1));
+  count_launch();
+  return backward ? launch_gradient<T>(logits, logits, w.coefs, rows, V, ld, s) : LLMK_OK;
+}
+
+template <typename T>
+int preference_finish_t(void* logits, const float2* stats, const PreferenceArgs& a, int pairs, int Tlen, int V, int ld,
+                        int backward, void* scratch, cudaStream_t s) {
+  const int rows = 2 * pairs * Tlen;
+  const Scratch w = split(scratch, rows);
+  LLMK_TRY(launch_fold<T>(w.sums, stats, logits, a.targets, rows, V, ld, s));
+  RowCoef* coefs = backward ? w.coefs : nullptr;
+  LLMK_CUDA(launch_after(preference_pair_kernel<T>, pairs, kPairThreads, 0, s, coefs, w.sums,
+                         static_cast<const T*>(logits), a, pairs, Tlen, V, ld, 1));
+  count_launch();
+  return backward ? launch_gradient<T>(logits, logits, w.coefs, rows, V, ld, s) : LLMK_OK;
+}
+
 }  // namespace
+
+int policy_finish(void* logits, llmk_dtype dtype, const float2* stats, const PolicyArgs& a, int rows, int V, int ld,
+                  int backward, void* scratch, cudaStream_t s) {
+  return dtype == LLMK_BF16 ? policy_finish_t<__nv_bfloat16>(logits, stats, a, rows, V, ld, backward, scratch, s)
+                            : policy_finish_t<float>(logits, stats, a, rows, V, ld, backward, scratch, s);
+}
+
+int preference_finish(void* logits, llmk_dtype dtype, const float2* stats, const PreferenceArgs& a, int pairs, int T, int V,
+                      int ld, int backward, void* scratch, cudaStream_t s) {
+  return dtype == LLMK_BF16
+             ? preference_finish_t<__nv_bfloat16>(logits, stats, a, pairs, T, V, ld, backward, scratch, s)
+             : preference_finish_t<float>(logits, stats, a, pairs, T, V, ld, backward, scratch, s);
+}
+
+int logps_finish(float* logps, const void* logits, llmk_dtype dtype, const float2* stats, const int* targets, int rows, int V,
+                 int ld, void* scratch, cudaStream_t s) {
+  const Scratch w = split(scratch, rows);
+  if (dtype == LLMK_BF16) LLMK_TRY(launch_fold<__nv_bfloat16>(w.sums, stats, logits, targets, rows, V, ld, s));
+  else LLMK_TRY(launch_fold<float>(w.sums, stats, logits, targets, rows, V, ld, s));
+  LLMK_CUDA(launch_after(logps_kernel, div_up(rows, 256), 256, 0, s, logps, w.sums, rows));
+  count_launch();
+  return LLMK_OK;
+}
+
+int sum_losses(float* out, const float* x, int n, float div, cudaStream_t s) {
+  sum_losses_kernel<<<1, 1024, 0, s>>>(out, x, n, div);
+  count_launch();
+  LLMK_CUDA(cudaGetLastError());
+  return LLMK_OK;
+}
+
+int check_policy(const char* what, const PolicyArgs& a, int rows) {
+  const std::string w = what;
+  if (!a.losses || !a.targets || !a.advantages || rows <= 0)
+    return fail(LLMK_ERR_INVALID_ARG, w + ": null operand or no rows");
+  if (bad_nonneg(a.clip_low) || bad_nonneg(a.clip_high) || a.clip_low > 1.f || !std::isfinite(a.kl_coef) ||
+      !std::isfinite(a.dscale))
+    return fail(LLMK_ERR_INVALID_ARG, w + ": clip_low in [0, 1], clip_high >= 0, finite kl_coef and dscale");
+  if (!a.ref_logps && (a.kl_coef != 0.f || a.kls))
+    return fail(LLMK_ERR_INVALID_ARG, w + ": the KL term needs ref_logps");
+  return LLMK_OK;
+}
+
+int check_preference(const char* what, const PreferenceArgs& a, int pairs, int T) {
+  const std::string w = what;
+  if (!a.losses || !a.targets || pairs <= 0 || T <= 0)
+    return fail(LLMK_ERR_INVALID_ARG, w + ": null operand, no pairs or no positions");
+  if (!(a.beta > 0.f) || std::isinf(a.beta) || !(a.smoothing >= 0.f) || a.smoothing > 1.f || !std::isfinite(a.dscale))
+    return fail(LLMK_ERR_INVALID_ARG, w + ": beta > 0, label_smoothing in [0, 1], finite dscale");
+  return LLMK_OK;
+}
+
 }  // namespace llmk
 
 using namespace llmk;
@@ -1067,14 +1206,10 @@ int llmk_policy_loss(float* losses, float* kls, float* logps, void* dlogits, con
                      const int* targets, const float* weights, const float* advantages, const float* old_logps,
                      const float* ref_logps, int rows, int V, int Vp, float clip_low, float clip_high, float kl_coef,
                      float dscale, void* workspace, size_t workspace_bytes, void* stream) {
-  if (!losses || !logits || !targets || !advantages || rows <= 0)
-    return fail(LLMK_ERR_INVALID_ARG, "policy_loss: null operand or no rows");
-  if (bad_nonneg(clip_low) || bad_nonneg(clip_high) || clip_low > 1.f || !std::isfinite(kl_coef) || !std::isfinite(dscale))
-    return fail(LLMK_ERR_INVALID_ARG, "policy_loss: clip_low in [0, 1], clip_high >= 0, finite kl_coef and dscale");
-  if (!ref_logps && (kl_coef != 0.f || kls))
-    return fail(LLMK_ERR_INVALID_ARG, "policy_loss: the KL term needs ref_logps");
-  LLMK_TRY(check_rows("policy_loss", dlogits, logits, dtype, rows, V, Vp, workspace, workspace_bytes));
   const PolicyArgs a{losses, kls, logps, targets, weights, advantages, old_logps, ref_logps, clip_low, clip_high, kl_coef, dscale};
+  if (!logits) return fail(LLMK_ERR_INVALID_ARG, "policy_loss: null operand or no rows");
+  LLMK_TRY(check_policy("policy_loss", a, rows));
+  LLMK_TRY(check_rows("policy_loss", dlogits, logits, dtype, rows, V, Vp, workspace, workspace_bytes));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return dtype == LLMK_BF16 ? policy_loss<__nv_bfloat16>(dlogits, logits, a, rows, V, Vp, workspace, s)
                             : policy_loss<float>(dlogits, logits, a, rows, V, Vp, workspace, s);
@@ -1088,12 +1223,10 @@ int llmk_preference_loss(float* losses, float* rewards, float* logps, void* dlog
                          const int* targets, const float* weights, const float* ref_logps, int pairs, int T, int V,
                          int Vp, float beta, float label_smoothing, float dscale, void* workspace,
                          size_t workspace_bytes, void* stream) {
-  if (!losses || !logits || !targets || pairs <= 0 || T <= 0)
-    return fail(LLMK_ERR_INVALID_ARG, "preference_loss: null operand, no pairs or no positions");
-  if (!(beta > 0.f) || std::isinf(beta) || !(label_smoothing >= 0.f) || label_smoothing > 1.f || !std::isfinite(dscale))
-    return fail(LLMK_ERR_INVALID_ARG, "preference_loss: beta > 0, label_smoothing in [0, 1], finite dscale");
-  LLMK_TRY(check_rows("preference_loss", dlogits, logits, dtype, 2LL * pairs * T, V, Vp, workspace, workspace_bytes));
   const PreferenceArgs a{losses, rewards, logps, targets, weights, ref_logps, beta, label_smoothing, dscale};
+  if (!logits) return fail(LLMK_ERR_INVALID_ARG, "preference_loss: null operand, no pairs or no positions");
+  LLMK_TRY(check_preference("preference_loss", a, pairs, T));
+  LLMK_TRY(check_rows("preference_loss", dlogits, logits, dtype, 2LL * pairs * T, V, Vp, workspace, workspace_bytes));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return dtype == LLMK_BF16 ? preference_loss<__nv_bfloat16>(dlogits, logits, a, pairs, T, V, Vp, workspace, s)
                             : preference_loss<float>(dlogits, logits, a, pairs, T, V, Vp, workspace, s);

@@ -144,6 +144,10 @@ struct llmk_gpt2 {
   const int *graph_in = nullptr, *graph_tg = nullptr;
   unsigned long long graph_launches = 0;  // kernels one replay runs
   float* hp_dev = nullptr;  // AdamW hyperparameters read by the captured update
+  // gradient clipping (llmk_gpt2_set_grad_clip): the largest norm, 0 = off, and
+  // the norm of the last update's gradients
+  float max_norm = 0.f;
+  float* grad_norm = nullptr;
 };
 
 namespace {
@@ -158,11 +162,11 @@ int ensure_device(llmk_gpt2* g) { return llmk::cuda_check(cudaSetDevice(g->devic
 // input gradient, layer weight gradient, and all three forms of the tied
 // lm_head.
 enum KClass { KC_GEMM_FWD = 0, KC_GEMM_DINP, KC_GEMM_DW, KC_GEMM_LMHEAD, KC_ATTN_FWD, KC_ATTN_BWD, KC_LN_FWD,
-              KC_LN_BWD, KC_XENT, KC_COLSUM, KC_ADAMW, KC_ENCODER, KC_CAST, KC_OTHER, KC_COUNT };
+              KC_LN_BWD, KC_XENT, KC_COLSUM, KC_ADAMW, KC_ENCODER, KC_CAST, KC_GRAD_NORM, KC_OTHER, KC_COUNT };
 const char* const kClassName[KC_COUNT] = {"gemm_fwd", "gemm_dinp", "gemm_dweight", "gemm_lm_head", "attention_fwd",
                                           "attention_bwd", "layernorm_fwd", "layernorm_bwd", "softmax_xent", "colsum",
-                                          "adamw", "encoder", "cast", "other"};
-const int kClassUnit[KC_COUNT] = {0, 0, 0, 0, 0, 0, 1, 1, 1, 1, 1, 1, 1, 1};  // 0 flop, 1 byte
+                                          "adamw", "encoder", "cast", "grad_norm", "other"};
+const int kClassUnit[KC_COUNT] = {0, 0, 0, 0, 0, 0, 1, 1, 1, 1, 1, 1, 1, 1, 1};  // 0 flop, 1 byte
 
 int timing_event(llmk_gpt2* g) {
   if (g->tev_used == g->tev.size()) {
@@ -291,7 +295,7 @@ void free_all(llmk_gpt2* g) {
   if (g->h2d_done) cudaEventDestroy(g->h2d_done);
   for (auto e : g->tev) cudaEventDestroy(e);
   if (g->graph_exec) cudaGraphExecDestroy(g->graph_exec);
-  f(g->hp_dev);
+  f(g->hp_dev); f(g->grad_norm);
   if (g->comm) ncclCommDestroy(g->comm);
   if (g->comm_stream) cudaStreamDestroy(g->comm_stream);
   if (g->aux_stream) cudaStreamDestroy(g->aux_stream);
@@ -299,6 +303,15 @@ void free_all(llmk_gpt2* g) {
     if (e) cudaEventDestroy(e);
   f(g->workspace2);
   if (g->own_stream && g->stream) cudaStreamDestroy(g->stream);
+}
+
+// All gradients as the one tensor they are.
+llmk_tensor flat_grads(const llmk_gpt2* g) {
+  return llmk_tensor{g->grads, nullptr, static_cast<long long>(g->nparams), LLMK_F32, LLMK_F32};
+}
+size_t grad_norm_bytes(const llmk_gpt2* g) {
+  const llmk_tensor t = flat_grads(g);
+  return llmk_grad_norm_workspace(&t, 1);
 }
 
 int alloc_all(llmk_gpt2* g) {
@@ -337,7 +350,8 @@ int alloc_all(llmk_gpt2* g) {
   if (bf) LLMK_TRY(dalloc(&g->dres_bf16, BT * C));
   LLMK_TRY(aalloc(&g->datty, BT * C)); LLMK_TRY(aalloc(&g->dqkv, BT * 3 * C)); LLMK_TRY(aalloc(&g->dfch, BT * 4 * C));
   LLMK_TRY(dalloc(&g->inputs, BT)); LLMK_TRY(dalloc(&g->targets, BT));
-  LLMK_TRY(dalloc(&g->hp_dev, 8));
+  LLMK_TRY(dalloc(&g->hp_dev, 8)); LLMK_TRY(dalloc(&g->grad_norm, 1));
+  LLMK_CUDA(cudaMemset(g->grad_norm, 0, sizeof(float)));
   LLMK_CUDA(cudaMallocHost(reinterpret_cast<void**>(&g->h_inputs), BT * sizeof(int)));
   LLMK_CUDA(cudaMallocHost(reinterpret_cast<void**>(&g->h_targets), BT * sizeof(int)));
   LLMK_CUDA(cudaMallocHost(reinterpret_cast<void**>(&g->h_loss), sizeof(float)));
@@ -349,7 +363,8 @@ int alloc_all(llmk_gpt2* g) {
   ws = std::max(ws, llmk_gemm_workspace(iVp, iC, iBT, g->math));
   ws = std::max(ws, llmk_layernorm_backward_workspace(iBT, iC));
   ws = std::max(ws, llmk_attention_backward_workspace(g->B, g->T, 3 * iC, static_cast<int>(NH)));
-  ws = std::max(ws, llmk::rowstats_bytes(iBT, iVp));
+  ws = std::max(ws, llmk_matmul_finetune_workspace(iBT, iVp));
+  ws = std::max(ws, grad_norm_bytes(g));
   ws = std::max(ws, llmk_encoder_backward_workspace(g->B, g->T));
   g->workspace_bytes = ws;
   LLMK_CUDA(cudaMalloc(&g->workspace, std::max<size_t>(ws, 256)));
@@ -555,10 +570,11 @@ struct StepOps {
 };
 }  // namespace
 
-int llmk_gpt2_forward(llmk_gpt2* g, const int* d_inputs, const int* d_targets) {
-  if (!g || !d_inputs) return fail(LLMK_ERR_INVALID_ARG, "gpt2_forward: null argument");
+// Tokens to the final LayerNorm (the lm_head's input) in g->lnf; the targets, if
+// given, to g->targets.
+static int forward_body(llmk_gpt2* g, const int* d_inputs, const int* d_targets) {
   const int B = g->B, T = g->T, C = g->cfg.channels, NH = g->cfg.num_heads, L = g->cfg.num_layers;
-  const int V = g->cfg.vocab_size, Vp = g->cfg.padded_vocab_size, BT = B * T;
+  const int BT = B * T;
   cudaStream_t s = g->stream;
   const float* P = g->params;
   const llmk_math mm = g->math;
@@ -572,7 +588,6 @@ int llmk_gpt2_forward(llmk_gpt2* g, const int* d_inputs, const int* d_targets) {
   };
   const int aux_f32 = bf ? 0 : LLMK_EPI_AUX_F32;
   if (d_inputs != g->inputs) LLMK_CUDA(cudaMemcpyAsync(g->inputs, d_inputs, BT * sizeof(int), cudaMemcpyDeviceToDevice, s));
-  g->have_targets = d_targets != nullptr;
   if (d_targets && d_targets != g->targets)
     LLMK_CUDA(cudaMemcpyAsync(g->targets, d_targets, BT * sizeof(int), cudaMemcpyDeviceToDevice, s));
   // encoder (gpt2cuda.cu:313)
@@ -613,29 +628,112 @@ int llmk_gpt2_forward(llmk_gpt2* g, const int* d_inputs, const int* d_targets) {
                      0));
     x = a.res3;
   }
-  LLMK_TRY(op.ln_fwd(g->lnf, adt, g->lnf_mean, g->lnf_rstd, x, P + g->off_lnfw, P + g->off_lnfb, BT, C));
+  return op.ln_fwd(g->lnf, adt, g->lnf_mean, g->lnf_rstd, x, P + g->off_lnfw, P + g->off_lnfb, BT, C);
+}
+
+// The lm_head weight as a GEMM operand: the bf16 mirror in bf16 mode, the fp32
+// master in tf32 mode.
+static const void* head_weight(const llmk_gpt2* g) {
+  return g->math == LLMK_MATH_BF16 ? static_cast<const void*>(g->params_bf16 + g->off_wte)
+                                   : static_cast<const void*>(g->params + g->off_wte);
+}
+
+// Logits and their per-slot softmax statistics (in the workspace, free during
+// the forward).
+static int head_rowstats(llmk_gpt2* g) {
+  const int C = g->cfg.channels, V = g->cfg.vocab_size, Vp = g->cfg.padded_vocab_size, BT = g->B * g->T;
+  TimedScope ts(g, KC_GEMM_LMHEAD, 2.0 * BT * static_cast<double>(Vp) * C);
+  return llmk::gemm_rowstats(g->logits, g->adt, Vp, g->lnf, C, head_weight(g), C, g->math, BT, Vp, C, nullptr,
+                             static_cast<float2*>(g->workspace), V, g->stream);
+}
+// The workspace behind the statistics.
+static void* head_scratch(llmk_gpt2* g) {
+  return static_cast<char*>(g->workspace) + (llmk::rowstats_bytes(g->B * g->T, g->cfg.padded_vocab_size) + 15) / 16 * 16;
+}
+// Bytes of the pass from logits to their gradient (both read and written once).
+static double head_pass_bytes(const llmk_gpt2* g) {
+  const int Vp = g->cfg.padded_vocab_size, BT = g->B * g->T;
+  return 2.0 * BT * static_cast<double>(Vp) * g->ae + llmk::rowstats_bytes(BT, Vp) + 8.0 * BT;
+}
+
+int llmk_gpt2_forward(llmk_gpt2* g, const int* d_inputs, const int* d_targets) {
+  if (!g || !d_inputs) return fail(LLMK_ERR_INVALID_ARG, "gpt2_forward: null argument");
+  const int C = g->cfg.channels, V = g->cfg.vocab_size, Vp = g->cfg.padded_vocab_size, BT = g->B * g->T;
+  cudaStream_t s = g->stream;
+  LLMK_TRY(forward_body(g, d_inputs, d_targets));
+  g->have_targets = d_targets != nullptr;
   // tied lm_head (gpt2cuda.cu:323): logits[BT, Vp] = lnf * wte^T, no bias
   if (!g->have_targets) {
-    LLMK_TRY(op.gemm(KC_GEMM_LMHEAD, g->logits, adt, Vp, g->lnf, 0, C, W(g->off_wte), 0, C, BT, Vp, C, nullptr, nullptr, 0));
-    return LLMK_OK;
+    const StepOps op{g, s, g->math, static_cast<double>(g->ae)};
+    return op.gemm(KC_GEMM_LMHEAD, g->logits, g->adt, Vp, g->lnf, 0, C, head_weight(g), 0, C, BT, Vp, C, nullptr, nullptr, 0);
   }
   // With targets, the lm_head GEMM's epilogue also reduces each row to
-  // per-slot softmax statistics (in the workspace, free during the forward),
-  // and one pass over the logits gives the losses and overwrites the logits
-  // with dlogits = (softmax - onehot) / (B*T) (gpt2cuda.cu:325,398).
-  auto* stats = static_cast<float2*>(g->workspace);
+  // per-slot softmax statistics, and one pass over the logits gives the losses
+  // and overwrites the logits with dlogits = (softmax - onehot) / (B*T)
+  // (gpt2cuda.cu:325,398).
+  LLMK_TRY(head_rowstats(g));
   {
-    TimedScope ts(g, KC_GEMM_LMHEAD, 2.0 * BT * static_cast<double>(Vp) * C);
-    LLMK_TRY(llmk::gemm_rowstats(g->logits, adt, Vp, g->lnf, C, W(g->off_wte), C, g->math, BT, Vp, C, nullptr, stats,
-                                 V, s));
-  }
-  {
-    TimedScope ts(g, KC_XENT, 2.0 * BT * static_cast<double>(Vp) * g->ae + llmk::rowstats_bytes(BT, Vp) + 8.0 * BT);
-    LLMK_TRY(llmk::rowstats_finish(0, g->losses, g->logits, g->logits, adt, stats, g->targets, BT, V, Vp,
-                                   1.0f / static_cast<float>(BT), 1, s));
+    TimedScope ts(g, KC_XENT, head_pass_bytes(g));
+    LLMK_TRY(llmk::rowstats_finish(0, g->losses, g->logits, g->logits, g->adt, static_cast<float2*>(g->workspace),
+                                   g->targets, BT, V, Vp, 1.0f / static_cast<float>(BT), 1, s));
   }
   TimedScope ts(g, KC_OTHER, 4.0 * BT);
   LLMK_TRY(llmk_mean(g->loss, g->losses, BT, s));
+  return LLMK_OK;
+}
+
+int llmk_gpt2_logprobs(llmk_gpt2* g, const int* d_inputs, const int* d_targets, float* d_logps) {
+  if (!g || !d_inputs || !d_targets || !d_logps) return fail(LLMK_ERR_INVALID_ARG, "gpt2_logprobs: null argument");
+  const int BT = g->B * g->T;
+  g->have_targets = false;  // the logits are no gradient: nothing for a backward
+  LLMK_TRY(forward_body(g, d_inputs, d_targets));
+  LLMK_TRY(head_rowstats(g));
+  TimedScope ts(g, KC_XENT, static_cast<double>(llmk::rowstats_bytes(BT, g->cfg.padded_vocab_size)) + 12.0 * BT);
+  return llmk::logps_finish(d_logps, g->logits, g->adt, static_cast<float2*>(g->workspace), g->targets, BT,
+                            g->cfg.vocab_size, g->cfg.padded_vocab_size, head_scratch(g), g->stream);
+}
+
+int llmk_gpt2_forward_policy(llmk_gpt2* g, const int* d_inputs, const int* d_targets, const float* weights,
+                             const float* advantages, const float* old_logps, const float* ref_logps, float clip_low,
+                             float clip_high, float kl_coef, float* kls, float* logps) {
+  if (!g || !d_inputs || !d_targets) return fail(LLMK_ERR_INVALID_ARG, "gpt2_forward_policy: null argument");
+  const int BT = g->B * g->T, V = g->cfg.vocab_size, Vp = g->cfg.padded_vocab_size;
+  const llmk::PolicyArgs a{g->losses, kls, logps, g->targets, weights, advantages, old_logps, ref_logps,
+                           clip_low, clip_high, kl_coef, 1.f};
+  LLMK_TRY(llmk::check_policy("gpt2_forward_policy", a, BT));
+  g->have_targets = false;
+  LLMK_TRY(forward_body(g, d_inputs, d_targets));
+  LLMK_TRY(head_rowstats(g));
+  {
+    TimedScope ts(g, KC_XENT, head_pass_bytes(g));
+    LLMK_TRY(llmk::policy_finish(g->logits, g->adt, static_cast<float2*>(g->workspace), a, BT, V, Vp, 1, head_scratch(g),
+                                 g->stream));
+  }
+  TimedScope ts(g, KC_OTHER, 4.0 * BT);
+  LLMK_TRY(llmk::sum_losses(g->loss, g->losses, BT, 1.f, g->stream));
+  g->have_targets = true;
+  return LLMK_OK;
+}
+
+int llmk_gpt2_forward_preference(llmk_gpt2* g, const int* d_inputs, const int* d_targets, const float* weights,
+                                 const float* ref_logps, float beta, float label_smoothing, float* rewards, float* logps) {
+  if (!g || !d_inputs || !d_targets) return fail(LLMK_ERR_INVALID_ARG, "gpt2_forward_preference: null argument");
+  if (g->B % 2) return fail(LLMK_ERR_INVALID_ARG, "gpt2_forward_preference: B must be even (pairs of sequences)");
+  const int pairs = g->B / 2, V = g->cfg.vocab_size, Vp = g->cfg.padded_vocab_size;
+  const llmk::PreferenceArgs a{g->losses, rewards, logps, g->targets, weights, ref_logps, beta, label_smoothing,
+                               1.f / static_cast<float>(pairs)};
+  LLMK_TRY(llmk::check_preference("gpt2_forward_preference", a, pairs, g->T));
+  g->have_targets = false;
+  LLMK_TRY(forward_body(g, d_inputs, d_targets));
+  LLMK_TRY(head_rowstats(g));
+  {
+    TimedScope ts(g, KC_XENT, head_pass_bytes(g));
+    LLMK_TRY(llmk::preference_finish(g->logits, g->adt, static_cast<float2*>(g->workspace), a, pairs, g->T, V, Vp, 1,
+                                     head_scratch(g), g->stream));
+  }
+  TimedScope ts(g, KC_OTHER, 4.0 * pairs);
+  LLMK_TRY(llmk::sum_losses(g->loss, g->losses, pairs, static_cast<float>(pairs), g->stream));
+  g->have_targets = true;
   return LLMK_OK;
 }
 
@@ -783,8 +881,10 @@ int llmk_gpt2_backward(llmk_gpt2* g) {
 // Under data parallelism it runs in two ranges: every parameter but the
 // embeddings as soon as their buckets are reduced, then wte / wpe once
 // their bucket is — so that update overlaps the embedding all-reduce, the
-// one the backward cannot hide. hp: the hyperparameters in device memory
-// (the form a captured graph replays), or nullptr to pass them by value.
+// one the backward cannot hide. With clipping on, the norm of all gradients comes
+// first and AdamW scales them on the way in. hp: the hyperparameters in device
+// memory (the form a captured graph replays, and clipping reads), or nullptr to
+// pass them by value.
 static int adamw_ranges(llmk_gpt2* g, const float* hp, float lr, float beta1, float beta2, float eps,
                         float weight_decay, int t) {
   const float scale = 1.0f / static_cast<float>(g->world);
@@ -793,12 +893,26 @@ static int adamw_ranges(llmk_gpt2* g, const float* hp, float lr, float beta1, fl
     TimedScope ts(g, KC_ADAMW, static_cast<double>(end - begin) * (28.0 + (g->params_bf16 ? 2.0 : 0.0)));
     __nv_bfloat16* pb = g->params_bf16 ? g->params_bf16 + begin : nullptr;
     const long long n = static_cast<long long>(end - begin);
+    if (g->max_norm > 0.f)
+      return llmk_adamw_clipped(g->params + begin, pb, g->grads + begin, g->m + begin, g->v + begin, n, hp, g->grad_norm,
+                                g->max_norm, g->stream);
     if (hp)
       return llmk_adamw_device_hparams(g->params + begin, pb, g->grads + begin, g->m + begin, g->v + begin, n, hp,
                                        g->stream);
     return llmk_adamw(g->params + begin, pb, g->grads + begin, g->m + begin, g->v + begin, n, lr, beta1, beta2, eps,
                       weight_decay, t, scale, g->stream);
   };
+  if (g->max_norm > 0.f) {
+    // the norm is over every gradient: nothing is updated before the last one is
+    // reduced
+    if (g->world > 1) LLMK_CUDA(cudaStreamWaitEvent(g->stream, g->comm_done, 0));
+    {
+      TimedScope ts(g, KC_GRAD_NORM, 4.0 * static_cast<double>(g->nparams));
+      const llmk_tensor t = flat_grads(g);
+      LLMK_TRY(llmk_grad_norm(g->grad_norm, &t, 1, scale, g->workspace, g->workspace_bytes, g->stream));
+    }
+    return range(0, g->nparams);
+  }
   if (g->world <= 1) return range(0, g->nparams);
   const size_t emb_end = g->off_wpe + g->tsize[llmk::WPE];  // [wte | wpe] lead the flat buffer
   LLMK_CUDA(cudaStreamWaitEvent(g->stream, g->layers_reduced, 0));
@@ -809,9 +923,42 @@ static int adamw_ranges(llmk_gpt2* g, const float* hp, float lr, float beta1, fl
 
 static int update_device_hparams(llmk_gpt2* g) { return adamw_ranges(g, g->hp_dev, 0.f, 0.f, 0.f, 0.f, 0.f, 1); }
 
+// A step's AdamW values to device memory, copied from pageable memory (staged
+// before the call returns), ahead of the update on the same stream.
+static int copy_hparams(llmk_gpt2* g, float lr, float beta1, float beta2, float eps, float weight_decay, int t) {
+  float hp[8];
+  llmk_adamw_hparams(hp, lr, beta1, beta2, eps, weight_decay, t, 1.0f / static_cast<float>(g->world));
+  LLMK_CUDA(cudaMemcpyAsync(g->hp_dev, hp, sizeof(hp), cudaMemcpyHostToDevice, g->stream));
+  return LLMK_OK;
+}
+
+int llmk_gpt2_set_grad_clip(llmk_gpt2* g, float max_norm) {
+  if (!g || !(max_norm >= 0.f)) return fail(LLMK_ERR_INVALID_ARG, "gpt2_set_grad_clip: max_norm must be 0 (off) or above");
+  if (g->graph_exec && max_norm != g->max_norm) {  // the captured update is another one
+    LLMK_CUDA(cudaStreamSynchronize(g->stream));
+    cudaGraphExecDestroy(g->graph_exec);
+    g->graph_exec = nullptr;
+  }
+  g->max_norm = max_norm;
+  return LLMK_OK;
+}
+
+int llmk_gpt2_grad_norm(llmk_gpt2* g, float* host_norm) {
+  if (!g || !host_norm) return fail(LLMK_ERR_INVALID_ARG, "gpt2_grad_norm");
+  LLMK_CUDA(cudaMemcpyAsync(g->h_loss, g->grad_norm, sizeof(float), cudaMemcpyDeviceToHost, g->stream));
+  LLMK_CUDA(cudaStreamSynchronize(g->stream));
+  *host_norm = *g->h_loss;
+  return LLMK_OK;
+}
+
 int llmk_gpt2_update(llmk_gpt2* g, float lr, float beta1, float beta2, float eps, float weight_decay, int t) {
   if (!g || t < 1) return fail(LLMK_ERR_INVALID_ARG, "gpt2_update");
-  LLMK_TRY(adamw_ranges(g, nullptr, lr, beta1, beta2, eps, weight_decay, t));
+  if (g->max_norm > 0.f) {
+    LLMK_TRY(copy_hparams(g, lr, beta1, beta2, eps, weight_decay, t));
+    LLMK_TRY(update_device_hparams(g));
+  } else {
+    LLMK_TRY(adamw_ranges(g, nullptr, lr, beta1, beta2, eps, weight_decay, t));
+  }
   ++g->steps;
   return LLMK_OK;
 }
@@ -854,11 +1001,7 @@ int llmk_gpt2_step_device(llmk_gpt2* g, const int* d_inputs, const int* d_target
     LLMK_TRY(llmk_gpt2_backward(g));
     return llmk_gpt2_update(g, lr, beta1, beta2, eps, weight_decay, t);
   }
-  // this step's AdamW values, copied from pageable memory (staged before the
-  // call returns), ahead of the replay on the same stream
-  float hp[8];
-  llmk_adamw_hparams(hp, lr, beta1, beta2, eps, weight_decay, t, 1.0f / static_cast<float>(g->world));
-  LLMK_CUDA(cudaMemcpyAsync(g->hp_dev, hp, sizeof(hp), cudaMemcpyHostToDevice, g->stream));
+  LLMK_TRY(copy_hparams(g, lr, beta1, beta2, eps, weight_decay, t));
   if (!g->graph_exec || d_inputs != g->graph_in || d_targets != g->graph_tg) {
     if (g->graph_exec) {
       cudaGraphExecDestroy(g->graph_exec);

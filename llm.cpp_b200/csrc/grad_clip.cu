@@ -132,7 +132,9 @@ __global__ void __launch_bounds__(kThreads) grad_squares_kernel(double* __restri
                                                                 const __grid_constant__ TensorTable<kCap> tab) {
   __shared__ double red[kThreads / 32];
   double sum = 0.0;
-  for (int u = blockIdx.x; u < tab.units; u += gridDim.x) {
+  // from the end: what is read again next (to be scaled, or by AdamW) is read
+  // from the front, and finds the last units read here in L2
+  for (int u = tab.units - 1 - static_cast<int>(blockIdx.x); u >= 0; u -= static_cast<int>(gridDim.x)) {
     const TensorRef& t = tab.t[find_tensor(tab, u)];
     const long long e0 = static_cast<long long>(u - t.unit0) * kUnit;
     const int n = static_cast<int>(min(static_cast<long long>(kUnit), t.n - e0));
@@ -154,6 +156,7 @@ __device__ __forceinline__ float norm_of(const double* __restrict__ partial, int
 __global__ void __launch_bounds__(kThreads) grad_norm_kernel(float* __restrict__ norm, const double* __restrict__ partial,
                                                              int n, float scale) {
   __shared__ double red[kThreads / 32];
+  grid_wait();
   const float v = norm_of(partial, n, scale, red);
   if (threadIdx.x == 0) *norm = v;
 }
@@ -192,6 +195,7 @@ __global__ void __launch_bounds__(kThreads) grad_scale_kernel(float* __restrict_
                                                               int partials, float max_norm,
                                                               const __grid_constant__ TensorTable<kCap> tab) {
   __shared__ double red[kThreads / 32];
+  grid_wait();  // not released early: the blocks set up would take room from the sums (250 -> 276 us)
   const float v = norm_of(partial, partials, 1.f, red);
   if (blockIdx.x == 0 && threadIdx.x == 0) *norm = v;
   const float q = max_norm / (v + 1e-6f);
@@ -302,12 +306,16 @@ void fill(TensorTable<kCap>* tab, const llmk_tensor* tensors, const Span& s) {
   tab->units = s.units;
 }
 
-// f(table) with the smallest of three table capacities that holds the span: a
+// f(table) with the smallest of four table capacities that holds the span: a
 // launch copies its whole parameter block.
 template <typename F>
 void with_table(const llmk_tensor* tensors, const Span& s, F f) {
-  if (s.count <= 16) {
-    TensorTable<16> tab;
+  if (s.count <= 4) {
+    TensorTable<4> tab;
+    fill(&tab, tensors, s);
+    f(tab);
+  } else if (s.count <= 40) {
+    TensorTable<40> tab;
     fill(&tab, tensors, s);
     f(tab);
   } else if (s.count <= 160) {
@@ -323,14 +331,22 @@ void with_table(const llmk_tensor* tensors, const Span& s, F f) {
 
 // Squares of every tensor; returns the number of partials.
 int launch_squares(double* partial, const llmk_tensor* tensors, const std::vector<Span>& spans, cudaStream_t s) {
-  int at = 0;
-  for (const Span& sp : spans) {
-    const int grid = grid_of(sp);
-    with_table(tensors, sp, [&](const auto& tab) { grad_squares_kernel<<<grid, kThreads, 0, s>>>(partial + at, tab); });
+  int n = 0;
+  for (const Span& sp : spans) n += grid_of(sp);
+  int at = n;
+  for (auto sp = spans.rbegin(); sp != spans.rend(); ++sp) {
+    const int grid = grid_of(*sp);
+    at -= grid;
+    with_table(tensors, *sp, [&](const auto& tab) { grad_squares_kernel<<<grid, kThreads, 0, s>>>(partial + at, tab); });
     count_launch();
-    at += grid;
   }
-  return at;
+  return n;
+}
+
+template <int kCap>
+cudaError_t launch_scale(int grid, cudaStream_t s, float* norm, const double* partial, int partials, float max_norm,
+                         const TensorTable<kCap>& tab) {
+  return launch_after(grad_scale_kernel<kCap>, grid, kThreads, 0, s, norm, partial, partials, max_norm, tab);
 }
 
 size_t workspace_of(const std::vector<Span>& spans) {
@@ -366,7 +382,7 @@ int llmk_grad_norm(float* norm, const llmk_tensor* tensors, int count, float sca
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   auto* partial = static_cast<double*>(workspace);
   const int n = launch_squares(partial, tensors, spans, s);
-  grad_norm_kernel<<<1, kThreads, 0, s>>>(norm, partial, n, scale);
+  LLMK_CUDA(launch_after(grad_norm_kernel, 1, kThreads, 0, s, norm, partial, n, scale));
   count_launch();
   LLMK_CUDA(cudaGetLastError());
   return LLMK_OK;
@@ -382,12 +398,11 @@ int llmk_clip_grad_norm(float* norm, const llmk_tensor* tensors, int count, floa
   auto* partial = static_cast<double*>(workspace);
   const int n = launch_squares(partial, tensors, spans, s);
   for (const Span& sp : spans) {
-    with_table(tensors, sp, [&](const auto& tab) {
-      grad_scale_kernel<<<grid_of(sp), kThreads, 0, s>>>(norm, partial, n, max_norm, tab);
-    });
+    cudaError_t e = cudaSuccess;
+    with_table(tensors, sp, [&](const auto& tab) { e = launch_scale(grid_of(sp), s, norm, partial, n, max_norm, tab); });
+    LLMK_CUDA(e);
     count_launch();
   }
-  LLMK_CUDA(cudaGetLastError());
   return LLMK_OK;
 }
 

@@ -287,4 +287,56 @@ int llmk_matmul_crossentropy_forward(float* losses, void* logits, llmk_dtype dty
   return rowstats_finish(0, losses, logits, logits, dtype, stats, targets, BT, V, Vp, dscale, backward, s);
 }
 
+size_t llmk_matmul_finetune_workspace(int BT, int Vp) {
+  if (BT <= 0 || Vp <= 0) return 0;
+  return (rowstats_bytes(BT, Vp) + 15) / 16 * 16 + finetune_scratch_bytes(BT);
+}
+
+}  // extern "C"
+
+// What the two fused losses share: the checks, the GEMM with its row
+// statistics, and where the scratch behind those lies.
+static int finetune_logits(const char* what, void* logits, llmk_dtype dtype, const void* inp, const void* W,
+                           const float* bias, int BT, int C, int Vp, int V, llmk_math math, void* workspace,
+                           size_t workspace_bytes, cudaStream_t s, void** scratch) {
+  LLMK_TRY(check_lmhead(logits, dtype, inp, W, BT, C, Vp, V, math, workspace, workspace_bytes, what));
+  if (workspace_bytes < llmk_matmul_finetune_workspace(BT, Vp))
+    return fail(LLMK_ERR_WORKSPACE, std::string(what) + ": workspace missing or too small");
+  if (!aligned16(logits)) return fail(LLMK_ERR_UNSUPPORTED, std::string(what) + ": logits need 16-byte alignment");
+  LLMK_TRY(gemm_rowstats(logits, dtype, Vp, inp, C, W, C, math, BT, Vp, C, bias, static_cast<float2*>(workspace), V, s));
+  *scratch = static_cast<char*>(workspace) + (rowstats_bytes(BT, Vp) + 15) / 16 * 16;
+  return LLMK_OK;
+}
+
+extern "C" {
+
+int llmk_matmul_policy_forward(float* losses, float* kls, float* logps, void* logits, llmk_dtype dtype, const void* inp,
+                               const void* W, const float* bias, const int* targets, const float* weights,
+                               const float* advantages, const float* old_logps, const float* ref_logps, int BT, int C,
+                               int Vp, int V, float clip_low, float clip_high, float kl_coef, float dscale, int backward,
+                               llmk_math math, void* workspace, size_t workspace_bytes, void* stream) {
+  const PolicyArgs a{losses, kls, logps, targets, weights, advantages, old_logps, ref_logps, clip_low, clip_high, kl_coef, dscale};
+  LLMK_TRY(check_policy("matmul_policy", a, BT));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  void* scratch = nullptr;
+  LLMK_TRY(finetune_logits("matmul_policy", logits, dtype, inp, W, bias, BT, C, Vp, V, math, workspace, workspace_bytes, s,
+                           &scratch));
+  return policy_finish(logits, dtype, static_cast<float2*>(workspace), a, BT, V, Vp, backward, scratch, s);
+}
+
+int llmk_matmul_preference_forward(float* losses, float* rewards, float* logps, void* logits, llmk_dtype dtype,
+                                   const void* inp, const void* W, const float* bias, const int* targets,
+                                   const float* weights, const float* ref_logps, int pairs, int T, int C, int Vp, int V,
+                                   float beta, float label_smoothing, float dscale, int backward, llmk_math math,
+                                   void* workspace, size_t workspace_bytes, void* stream) {
+  const PreferenceArgs a{losses, rewards, logps, targets, weights, ref_logps, beta, label_smoothing, dscale};
+  LLMK_TRY(check_preference("matmul_preference", a, pairs, T));
+  if (2LL * pairs * T > (1 << 30)) return fail(LLMK_ERR_UNSUPPORTED, "matmul_preference: more than 2^30 rows");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  void* scratch = nullptr;
+  LLMK_TRY(finetune_logits("matmul_preference", logits, dtype, inp, W, bias, 2 * pairs * T, C, Vp, V, math, workspace,
+                           workspace_bytes, s, &scratch));
+  return preference_finish(logits, dtype, static_cast<float2*>(workspace), a, pairs, T, V, Vp, backward, scratch, s);
+}
+
 }  // extern "C"

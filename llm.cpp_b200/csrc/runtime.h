@@ -76,6 +76,60 @@ inline size_t rowstats_bytes(int rows, int ld) {
   return static_cast<size_t>((ld + 63) / 64) * rows * 8 + (static_cast<size_t>(rows) * 4 + 15) / 16 * 16;
 }
 
+// The fine-tuning losses from the slot statistics of a logits GEMM
+// (finetune_loss.cu): what gemm_rowstats left in `stats`, losses[row] or
+// losses[pair] and the optional outputs of the args, and with `backward` the
+// gradient over the logits. `scratch`: finetune_scratch_bytes(rows), 16-byte
+// aligned. logps_finish writes only the log-probabilities.
+struct PolicyArgs {
+  float *losses, *kls, *logps;
+  const int* targets;
+  const float *weights, *advantages, *old_logps, *ref_logps;
+  float clip_low, clip_high, kl_coef, dscale;
+};
+struct PreferenceArgs {
+  float *losses, *rewards, *logps;
+  const int* targets;
+  const float *weights, *ref_logps;
+  float beta, smoothing, dscale;
+};
+inline size_t finetune_scratch_bytes(int rows) { return static_cast<size_t>(rows) * 32; }
+int policy_finish(void* logits, llmk_dtype dtype, const float2* stats, const PolicyArgs& a, int rows, int V, int ld,
+                  int backward, void* scratch, cudaStream_t stream);
+int preference_finish(void* logits, llmk_dtype dtype, const float2* stats, const PreferenceArgs& a, int pairs, int T, int V,
+                      int ld, int backward, void* scratch, cudaStream_t stream);
+int logps_finish(float* logps, const void* logits, llmk_dtype dtype, const float2* stats, const int* targets, int rows, int V,
+                 int ld, void* scratch, cudaStream_t stream);
+// *out = sum(x[0..n)) / div, in a fixed order.
+int sum_losses(float* out, const float* x, int n, float div, cudaStream_t stream);
+// The refusals of the two losses' entry points (LLMK_OK when there is none).
+int check_policy(const char* what, const PolicyArgs& a, int rows);
+int check_preference(const char* what, const PreferenceArgs& a, int pairs, int T);
+
+#ifdef __CUDACC__
+// Launches a kernel that may be set up while the one before it in the stream
+// still runs (programmatic dependent launch). The kernel calls grid_wait()
+// before it touches memory, which waits until that one has finished and its
+// writes are visible; the one before calls grid_release() to let the set-up
+// begin. Every kernel of such a chain waits, so each also follows all before.
+template <typename... Params, typename... Args>
+cudaError_t launch_after(void (*kernel)(Params...), int grid, int block, size_t smem, cudaStream_t s, Args... args) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+#endif
+
 }  // namespace llmk
 
 #define LLMK_TRY(expr)            \

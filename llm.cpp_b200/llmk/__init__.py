@@ -103,6 +103,11 @@ SIGNATURES: dict[str, tuple] = {
                                vp]),
     "llmk_preference_loss_workspace": (sz, [i32, i32, i32]),
     "llmk_preference_loss": (i32, [vp, vp, vp, vp, vp, i32, vp, vp, vp, i32, i32, i32, i32, f32, f32, f32, vp, sz, vp]),
+    "llmk_matmul_finetune_workspace": (sz, [i32, i32]),
+    "llmk_matmul_policy_forward": (i32, [vp, vp, vp, vp, i32, vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, f32, f32,
+                                         f32, f32, i32, i32, vp, sz, vp]),
+    "llmk_matmul_preference_forward": (i32, [vp, vp, vp, vp, i32, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, f32, f32,
+                                             f32, i32, i32, vp, sz, vp]),
     "llmk_grad_norm_workspace": (sz, [vp, i32]),
     "llmk_grad_norm": (i32, [vp, vp, i32, f32, vp, sz, vp]),
     "llmk_clip_grad_norm": (i32, [vp, vp, i32, f32, vp, sz, vp]),
@@ -119,6 +124,11 @@ SIGNATURES: dict[str, tuple] = {
     "llmk_gpt2_read_gradients": (i32, [vp, vp, sz]),
     "llmk_gpt2_set_train_data": (i32, [vp, vp, vp]),
     "llmk_gpt2_forward": (i32, [vp, vp, vp]),
+    "llmk_gpt2_logprobs": (i32, [vp, vp, vp, vp]),
+    "llmk_gpt2_forward_policy": (i32, [vp, vp, vp, vp, vp, vp, vp, f32, f32, f32, vp, vp]),
+    "llmk_gpt2_forward_preference": (i32, [vp, vp, vp, vp, vp, f32, f32, vp, vp]),
+    "llmk_gpt2_set_grad_clip": (i32, [vp, f32]),
+    "llmk_gpt2_grad_norm": (i32, [vp, C.POINTER(f32)]),
     "llmk_gpt2_zero_grad": (i32, [vp]),
     "llmk_gpt2_backward": (i32, [vp]),
     "llmk_gpt2_update": (i32, [vp, f32, f32, f32, f32, f32, i32]),
@@ -191,8 +201,12 @@ def ptr(t) -> int | None:
 
 def stream_ptr(stream=None) -> int | None:
     import torch
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return s.cuda_stream
+    if stream is not None:
+        return stream.cuda_stream
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # 0.2 us; the stream object below takes 3
+    if raw is not None:
+        return raw(torch.cuda.current_device())
+    return torch.cuda.current_stream().cuda_stream
 
 
 def dtype_code(t) -> int:
@@ -236,22 +250,22 @@ def _ws(workspace) -> tuple[int | None, int]:
 def _device_of(t) -> int:
     """Device index of t, which has to be the current CUDA device (the library launches there)."""
     import torch
-    if not t.is_cuda or t.get_device() != torch.cuda.current_device():
+    dev = t.get_device()
+    if dev < 0 or dev != torch.cuda.current_device():
         raise ValueError(f"expected a tensor on the current CUDA device, got one on {t.device}")
-    return t.get_device()
+    return dev
 
 
-def _check(what: str, dev: int, tensors) -> None:
-    """Each (name, tensor or None, dtype, element count): contiguous, of that type and size, on device dev."""
-    for name, t, dtype, n in tensors:
-        if t is None:
-            continue
-        if t.dtype is not dtype:
-            raise TypeError(f"{what}: {name} must be {dtype}, got {t.dtype}")
-        if t.numel() != n or not t.is_contiguous():
-            raise ValueError(f"{what}: {name} must be contiguous with {n} elements, got {tuple(t.shape)}")
-        if t.get_device() != dev:
-            raise ValueError(f"{what}: {name} is on another device than the logits or parameters")
+def _check(what: str, dev: int, dtype, n: int, **tensors) -> None:
+    """Each tensor (or None): of that type, contiguous with n elements, on device dev. A launch from Python is a few
+    microseconds; this is kept to four tests a tensor."""
+    for t in tensors.values():
+        if t is not None and (t.dtype is not dtype or t.numel() != n or t.get_device() != dev or not t.is_contiguous()):
+            name = next(k for k, v in tensors.items() if v is t)
+            if t.dtype is not dtype:
+                raise TypeError(f"{what}: {name} must be {dtype}, got {t.dtype}")
+            raise ValueError(f"{what}: {name} must be contiguous with {n} elements on the same device as the others, "
+                             f"got {tuple(t.shape)} on {t.device}")
 
 
 def policy_loss_workspace(rows: int, Vp: int) -> int:
@@ -263,15 +277,14 @@ def policy_loss(losses, logits, targets, advantages, *, V=None, weights=None, ol
                 logps=None, dlogits=None, clip_low=0.2, clip_high=0.2, kl_coef=0.0, dscale=1.0, workspace=None,
                 stream=None):
     """Clipped policy loss over logits (..., Vp), and its gradient when dlogits is given (llmk_policy_loss)."""
-    from torch import float32, int32
+    import torch
     Vp = logits.shape[-1]
     rows = logits.numel() // Vp
-    _check("policy_loss", _device_of(logits),
-           (("logits", logits, logits.dtype, rows * Vp), ("dlogits", dlogits, logits.dtype, rows * Vp),
-            ("targets", targets, int32, rows), ("losses", losses, float32, rows),
-            ("advantages", advantages, float32, rows), ("weights", weights, float32, rows),
-            ("old_logps", old_logps, float32, rows), ("ref_logps", ref_logps, float32, rows),
-            ("kls", kls, float32, rows), ("logps", logps, float32, rows)))
+    dev = _device_of(logits)
+    _check("policy_loss", dev, logits.dtype, rows * Vp, logits=logits, dlogits=dlogits)
+    _check("policy_loss", dev, torch.int32, rows, targets=targets)
+    _check("policy_loss", dev, torch.float32, rows, losses=losses, advantages=advantages, weights=weights,
+           old_logps=old_logps, ref_logps=ref_logps, kls=kls, logps=logps)
     ws, ws_bytes = _ws(workspace)
     call("llmk_policy_loss", ptr(losses), ptr(kls), ptr(logps), ptr(dlogits), ptr(logits), dtype_code(logits),
          ptr(targets), ptr(weights), ptr(advantages), ptr(old_logps), ptr(ref_logps), rows, Vp if V is None else V, Vp,
@@ -287,16 +300,17 @@ def preference_loss(losses, logits, targets, *, V=None, weights=None, ref_logps=
                     dlogits=None, beta=0.1, label_smoothing=0.0, dscale=1.0, workspace=None, stream=None):
     """Preference loss over losses.numel() pairs of sequences of logits (..., Vp), the preferred ones first, and its
     gradient when dlogits is given (llmk_preference_loss)."""
-    from torch import float32, int32
+    import torch
     Vp, pairs = logits.shape[-1], losses.numel()
     rows = logits.numel() // Vp
     if pairs == 0 or rows % (2 * pairs):
         raise ValueError(f"preference_loss: {rows} rows of logits are not {pairs} pairs of sequences")
-    _check("preference_loss", _device_of(logits),
-           (("logits", logits, logits.dtype, rows * Vp), ("dlogits", dlogits, logits.dtype, rows * Vp),
-            ("targets", targets, int32, rows), ("losses", losses, float32, pairs), ("weights", weights, float32, rows),
-            ("ref_logps", ref_logps, float32, 2 * pairs), ("rewards", rewards, float32, 2 * pairs),
-            ("logps", logps, float32, rows)))
+    dev = _device_of(logits)
+    _check("preference_loss", dev, logits.dtype, rows * Vp, logits=logits, dlogits=dlogits)
+    _check("preference_loss", dev, torch.int32, rows, targets=targets)
+    _check("preference_loss", dev, torch.float32, rows, weights=weights, logps=logps)
+    _check("preference_loss", dev, torch.float32, pairs, losses=losses)
+    _check("preference_loss", dev, torch.float32, 2 * pairs, ref_logps=ref_logps, rewards=rewards)
     ws, ws_bytes = _ws(workspace)
     call("llmk_preference_loss", ptr(losses), ptr(rewards), ptr(logps), ptr(dlogits), ptr(logits), dtype_code(logits),
          ptr(targets), ptr(weights), ptr(ref_logps), pairs, rows // (2 * pairs), Vp if V is None else V, Vp, beta,
@@ -331,21 +345,30 @@ def grad_norm_workspace(tensors: TensorList) -> int:
 
 def grad_norm(norm, tensors: TensorList, *, scale=1.0, workspace=None, stream=None):
     """norm[0] = |scale| * the 2-norm over all tensors (llmk_grad_norm)."""
+    import torch
+    _check("grad_norm", _device_of(norm), torch.float32, 1, norm=norm)
+    if tensors.device != norm.get_device():
+        raise ValueError("grad_norm: norm is on another device than the tensors")
     call("llmk_grad_norm", ptr(norm), tensors.array, len(tensors), scale, *_ws(workspace), stream_ptr(stream))
 
 
 def clip_grad_norm(norm, tensors: TensorList, max_norm, *, workspace=None, stream=None):
     """norm[0] as grad_norm, and every tensor scaled to a global norm of at most max_norm (llmk_clip_grad_norm)."""
+    import torch
+    _check("clip_grad_norm", _device_of(norm), torch.float32, 1, norm=norm)
+    if tensors.device != norm.get_device():
+        raise ValueError("clip_grad_norm: norm is on another device than the tensors")
     call("llmk_clip_grad_norm", ptr(norm), tensors.array, len(tensors), max_norm, *_ws(workspace), stream_ptr(stream))
 
 
 def adamw_clipped(params, grads, m, v, hparams, norm, max_norm, *, params_bf16=None, stream=None):
     """AdamW with device hyperparameters on gradients clipped by the norm in device memory (llmk_adamw_clipped)."""
-    from torch import bfloat16, float32
-    n = params.numel()
-    _check("adamw_clipped", _device_of(params),
-           (("params", params, float32, n), ("grads", grads, float32, n), ("m", m, float32, n), ("v", v, float32, n),
-            ("params_bf16", params_bf16, bfloat16, n), ("hparams", hparams, float32, 8), ("norm", norm, float32, 1)))
+    import torch
+    n, dev = params.numel(), _device_of(params)
+    _check("adamw_clipped", dev, torch.float32, n, params=params, grads=grads, m=m, v=v)
+    _check("adamw_clipped", dev, torch.bfloat16, n, params_bf16=params_bf16)
+    _check("adamw_clipped", dev, torch.float32, 8, hparams=hparams)
+    _check("adamw_clipped", dev, torch.float32, 1, norm=norm)
     call("llmk_adamw_clipped", ptr(params), ptr(params_bf16), ptr(grads), ptr(m), ptr(v), params.numel(), ptr(hparams),
          ptr(norm), max_norm, stream_ptr(stream))
 
@@ -445,6 +468,32 @@ class GPT2:
 
     def forward(self, d_inputs: int, d_targets: int | None):
         call("llmk_gpt2_forward", self.h, d_inputs, d_targets)
+
+    def logprobs(self, d_inputs: int, d_targets: int, d_logps: int):
+        """Log-probabilities of the targets into B*T device floats."""
+        call("llmk_gpt2_logprobs", self.h, d_inputs, d_targets, d_logps)
+
+    def forward_policy(self, d_inputs: int, d_targets: int, advantages: int, *, weights=None, old_logps=None,
+                       ref_logps=None, clip_low=0.2, clip_high=0.2, kl_coef=0.0, kls=None, logps=None):
+        """Forward with the clipped policy loss (device addresses of B*T floats); backward() follows."""
+        call("llmk_gpt2_forward_policy", self.h, d_inputs, d_targets, weights, advantages, old_logps, ref_logps, clip_low,
+             clip_high, kl_coef, kls, logps)
+
+    def forward_preference(self, d_inputs: int, d_targets: int, *, weights=None, ref_logps=None, beta=0.1,
+                           label_smoothing=0.0, rewards=None, logps=None):
+        """Forward with the preference loss over B/2 pairs, the preferred sequences first; backward() follows."""
+        call("llmk_gpt2_forward_preference", self.h, d_inputs, d_targets, weights, ref_logps, beta, label_smoothing, rewards,
+             logps)
+
+    def set_grad_clip(self, max_norm: float):
+        """Clip the global gradient norm in every later update (0: off)."""
+        call("llmk_gpt2_set_grad_clip", self.h, max_norm)
+
+    def grad_norm(self) -> float:
+        """Norm of the last clipped update's gradients before clipping."""
+        v = C.c_float(0.0)
+        call("llmk_gpt2_grad_norm", self.h, C.byref(v))
+        return v.value
 
     def backward(self):
         call("llmk_gpt2_backward", self.h)

@@ -144,3 +144,58 @@ def test_wrappers_check_their_tensors(llmk_lib):
     with pytest.raises(ValueError):
         llmk.TensorList([torch.zeros(4, 4).t()])
     assert C.sizeof(llmk.Tensor) == 32
+
+
+def matmul_policy(**kw):
+    a = dict(losses=A, kls=None, logps=None, logits=A, dtype=1, inp=A, W=A, bias=None, targets=A, weights=None,
+             advantages=A, old=None, ref=None, BT=8, C=64, Vp=104, V=100, lo=0.2, hi=0.2, kl=0.0, dscale=1.0, backward=1,
+             math=1, ws=A, ws_bytes=BIG, stream=None)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return tuple(a.values())
+
+
+def matmul_preference(**kw):
+    a = dict(losses=A, rewards=None, logps=None, logits=A, dtype=1, inp=A, W=A, bias=None, targets=A, weights=None,
+             ref=None, pairs=2, T=4, C=64, Vp=104, V=100, beta=0.1, smooth=0.0, dscale=1.0, backward=1, math=1, ws=A,
+             ws_bytes=BIG, stream=None)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return tuple(a.values())
+
+
+MATMUL = [(dict(losses=None), INVALID), (dict(targets=None), INVALID), (dict(logits=None), INVALID), (dict(inp=None), INVALID),
+          (dict(W=None), INVALID), (dict(C=0), INVALID), (dict(V=105), INVALID), (dict(dtype=2), INVALID),
+          (dict(math=3), INVALID), (dict(Vp=102), UNSUPPORTED), (dict(ws=None), WORKSPACE), (dict(ws_bytes=200), WORKSPACE),
+          (dict(dscale=float("nan")), INVALID)]
+
+
+@pytest.mark.parametrize("kw,code", MATMUL + [(dict(BT=0), INVALID), (dict(advantages=None), INVALID), (dict(kl=0.1), INVALID),
+                                              (dict(lo=2.0), INVALID)])
+def test_matmul_policy_refuses(llmk_lib, kw, code):
+    assert llmk_lib.llmk_matmul_policy_forward(*matmul_policy(**kw)) == code
+    assert b"matmul_policy" in llmk_lib.llmk_last_error()
+
+
+@pytest.mark.parametrize("kw,code", MATMUL + [(dict(pairs=0), INVALID), (dict(T=0), INVALID), (dict(beta=0.0), INVALID),
+                                              (dict(smooth=2.0), INVALID), (dict(pairs=1 << 20, T=1 << 20), UNSUPPORTED)])
+def test_matmul_preference_refuses(llmk_lib, kw, code):
+    assert llmk_lib.llmk_matmul_preference_forward(*matmul_preference(**kw)) == code
+    assert b"matmul_preference" in llmk_lib.llmk_last_error()
+
+
+def test_finetune_workspace(llmk_lib):
+    L = llmk_lib
+    assert L.llmk_matmul_finetune_workspace(0, 104) == 0
+    need = L.llmk_matmul_finetune_workspace(8, 104)
+    assert need >= L.llmk_matmul_softmax_workspace(8, 104) + 8 * 32
+    assert L.llmk_matmul_policy_forward(*matmul_policy(ws_bytes=need - 1)) == WORKSPACE
+
+
+def test_model_entry_points_refuse(llmk_lib):
+    L = llmk_lib
+    assert L.llmk_gpt2_logprobs(None, A, A, A) == INVALID
+    assert L.llmk_gpt2_forward_policy(None, A, A, None, A, None, None, 0.2, 0.2, 0.0, None, None) == INVALID
+    assert L.llmk_gpt2_forward_preference(None, A, A, None, None, 0.1, 0.0, None, None) == INVALID
+    assert L.llmk_gpt2_set_grad_clip(None, 1.0) == INVALID
+    assert L.llmk_gpt2_grad_norm(None, None) == INVALID
