@@ -66,26 +66,33 @@ __device__ __forceinline__ double warp_sum_d(double v) {
 // sum 0 (or NaN, when it holds one), not exp(-inf + inf).
 __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.f : m; }
 
-// max and sum of a row from its slots.
-__device__ __forceinline__ void fold_slots(const RowSum* __restrict__ slots, long long row, int rows, int nslots, float* m,
-                                           double* s) {
+// A row's sum from its slots, and its target's logit (NaN for a target outside
+// [0, V)). The loads do not wait for one another but for the logit, which needs
+// the target.
+constexpr int kMaxParts = 16;
+template <typename T>
+__device__ __forceinline__ RowSum fold_slots(const RowSum* __restrict__ slots, const T* logits, long long row, int rows,
+                                             int nslots, int target, int V, int ld) {
+  const float xt = target >= 0 && target < V ? elem_to_float(logits[row * ld + target]) : NAN;
+  if (nslots == 1) {
+    RowSum t = slots[row];
+    t.xt = xt;
+    return t;
+  }
+  RowSum p[kMaxParts];
+#pragma unroll
+  for (int k = 0; k < kMaxParts; ++k) p[k] = k < nslots ? slots[static_cast<long long>(k) * rows + row] : RowSum{0.0, -INFINITY, 0.f};
   float M = -INFINITY;
-  for (int k = 0; k < nslots; ++k) M = fmaxf(M, slots[static_cast<long long>(k) * rows + row].m);
+#pragma unroll
+  for (int k = 0; k < kMaxParts; ++k) M = fmaxf(M, p[k].m);
   const float ref = finite_max(M);
   double S = 0.0;
-  for (int k = 0; k < nslots; ++k) {
-    const RowSum p = slots[static_cast<long long>(k) * rows + row];
-    S += p.s * static_cast<double>(expf(p.m - ref));
-  }
-  *m = M;
-  *s = S;
+#pragma unroll
+  for (int k = 0; k < kMaxParts; ++k) S += p[k].s * static_cast<double>(expf(p[k].m - ref));
+  return RowSum{S, M, xt};
 }
-
-// lp of a row; NaN for a target outside [0, V).
-template <typename T>
-__device__ __forceinline__ double target_logp(const T* logits, long long row, int ld, int V, int target, float m, double s) {
-  if (target < 0 || target >= V) return static_cast<double>(NAN);
-  return static_cast<double>(elem_to_float(logits[row * ld + target])) - static_cast<double>(m) - log(s);
+__device__ __forceinline__ double logp_of(const RowSum& t) {
+  return static_cast<double>(t.xt) - static_cast<double>(t.m) - log(t.s);
 }
 
 // The policy loss of one live row, given lp: writes the row's outputs and
@@ -474,17 +481,29 @@ struct UnitWalk {
   }
 };
 
-// A CTA's rows, the live ones and the masked ones apart.
-constexpr int kMaxItems = 2048;  // rows of one CTA in one launch
+// A CTA's units, those of live rows and those of masked ones apart.
+constexpr int kMaxItems = 2048;  // units of one CTA in one launch
 constexpr int kRowWarps = 24;
 constexpr int kRowThreads = 32 * kRowWarps;
 struct RowList {
   uint16_t items[kMaxItems];  // the live ones from the front, the masked ones from the back
   uint8_t masked[kMaxItems];
   int count;
-  // Called by the whole CTA after each thread wrote its part of masked[]; returns
-  // the number of live ones.
-  __device__ __forceinline__ int sort(int n) {
+  // Called by the whole CTA with its n rows' flags; returns the number of live
+  // ones. Up to 32 rows every warp sorts for itself, and nobody waits.
+  template <typename F>
+  __device__ __forceinline__ int sort(int n, F is_masked) {
+    if (n <= 32) {
+      const int lane = threadIdx.x & 31;
+      const bool is_live = lane < n && !is_masked(lane);
+      const unsigned all = __ballot_sync(0xffffffffu, is_live);
+      const int at = __popc(all & ((1u << lane) - 1u));
+      if (is_live) items[at] = static_cast<uint16_t>(lane);  // the same values from every warp
+      else if (lane < n) items[n - 1 - (lane - at)] = static_cast<uint16_t>(lane);
+      __syncwarp();
+      return __popc(all);
+    }
+    for (int i = threadIdx.x; i < n; i += kRowThreads) masked[i] = is_masked(i);
     __syncthreads();
     if (threadIdx.x < 32) {
       const int lane = threadIdx.x;
@@ -509,14 +528,15 @@ struct RowList {
 
 enum RowMode { kRowGrad, kRowEval, kRowStats };
 
-// How row_kernel shares rows [row0, row1) of `rows` out. CTA b's rows are row0 +
-// b, row0 + b + grid, ...; a unit is a live row (kRowStats: one of `parts` parts
-// of it) of `vecs` vectors; `group` warps take a unit, each `seg` vectors of it,
-// through its ring in chunks of `sub`.
+// How row_kernel shares the work out. A unit is a row, or (kRowStats) one of
+// `parts` parts of it, of `vecs` vectors; a launch covers units [unit0, unit1) of
+// rows * parts, CTA b those at unit0 + b, unit0 + b + grid, ...; `group` warps
+// take a unit, each `seg` vectors of it, through its ring in chunks of `sub`.
 struct RowJob {
   RowSum* slots;
   const float* weights;
-  int rows, row0, row1, V, ld;
+  int rows, V, ld;
+  unsigned unit0, unit1;
   int parts, vecs, group, seg, sub, stages;
   unsigned int* status;
 };
@@ -541,16 +561,23 @@ __global__ void __launch_bounds__(kRowThreads, 1) row_kernel(T* dlogits, const T
   __shared__ int abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (kMode == kRowStats) grid_release();
-  const int first_row = job.row0 + blockIdx.x;
-  const int n_items = (job.row1 - first_row + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
-  auto row_of = [&](int item) { return first_row + static_cast<long long>(item) * gridDim.x; };
-  for (int i = threadIdx.x; i < n_items; i += kRowThreads) todo.masked[i] = job.weights && job.weights[row_of(i)] == 0.f;
+  const unsigned first = job.unit0 + blockIdx.x;
+  const int n_items = static_cast<int>((job.unit1 - first + gridDim.x - 1) / gridDim.x);
+  auto unit_of = [&](int item) { return first + static_cast<unsigned>(item) * gridDim.x; };
+  auto row_of = [&](int item) {
+    const unsigned u = unit_of(item);
+    return static_cast<long long>(kMode == kRowStats && job.parts > 1 ? u / static_cast<unsigned>(job.parts) : u);
+  };
+  auto part_of = [&](int item) {
+    return kMode == kRowStats && job.parts > 1 ? static_cast<int>(unit_of(item) % static_cast<unsigned>(job.parts)) : 0;
+  };
   if (threadIdx.x == 0) {
     for (int i = 0; i < kRowWarps * kMaxStages; ++i) mbar_init(bars + i, 1);
     abort_word = 0;
     fence_mbar_init();
   }
-  const int live = todo.sort(n_items);
+  const int live = todo.sort(n_items, [&](int i) { return job.weights && job.weights[row_of(i)] == 0.f; });
+  __syncthreads();
   const int G = job.group, group = warp / G, gw = warp - group * G;
   const int groups = kRowWarps / G;
   auto meet = [&] {
@@ -562,26 +589,30 @@ __global__ void __launch_bounds__(kRowThreads, 1) row_kernel(T* dlogits, const T
   ring.status = job.status;
   ring.abort_flag = &abort_word;
   const int row_vecs = (job.V + kV - 1) / kV;
-  UnitWalk at(group, groups, live, kMode == kRowStats ? job.parts : 1);
-  UnitWalk ahead = at;  // the unit whose chunks are loaded next
-  // this warp's vectors of a unit: the first one's number in the row, and how many
-  auto my_first = [&](const UnitWalk& u) { return u.part * job.vecs + gw * job.seg; };
-  auto my_count = [&](const UnitWalk& u) {
-    return max(0, min(job.seg, min(job.vecs, row_vecs - u.part * job.vecs) - gw * job.seg));
+  // this warp's vectors of part `part` of a row: the first one's number in the
+  // row, and how many
+  auto my_first = [&](int part) { return part * job.vecs + gw * job.seg; };
+  auto my_count = [&](int part) {
+    return max(0, min(job.seg, min(job.vecs, row_vecs - part * job.vecs) - gw * job.seg));
   };
 
-  // The copies run ahead of the work by what the ring holds.
-  int done = 0;  // vectors of `ahead` that are loaded or on their way
-  int count = my_count(ahead);
+  // The copies run ahead of the work by what the ring holds: `ahead` is the
+  // live item they are at, `done` of its `count` vectors are loaded or on their
+  // way.
+  int ahead = group, done = 0, count = 0;
+  const uint4* src = nullptr;
+  auto open_ahead = [&] {
+    if (ahead >= live) return;
+    const int item = todo.live(ahead), part = part_of(item);
+    done = 0;
+    count = my_count(part);
+    src = reinterpret_cast<const uint4*>(logits + row_of(item) * job.ld) + my_first(part);
+  };
+  open_ahead();
   auto load_next = [&] {
-    while (ahead.valid() && done >= count) {
-      ahead.next();
-      done = 0;
-      count = my_count(ahead);
-    }
-    if (!ahead.valid()) return;
-    const int n = min(job.sub, count - done);
-    ring.load(reinterpret_cast<const uint4*>(logits + row_of(todo.live(ahead.item)) * job.ld) + my_first(ahead) + done, n * 16, lane);
+    while (ahead < live && done >= count) ahead += groups, open_ahead();
+    if (ahead >= live) return;
+    ring.load(src + done, min(job.sub, count - done) * 16, lane);
     done += job.sub;
   };
   for (int i = 0; i < job.stages; ++i) load_next();
@@ -597,11 +628,10 @@ __global__ void __launch_bounds__(kRowThreads, 1) row_kernel(T* dlogits, const T
 
   bool ok = true;
   int k = 0;  // units so far
-  while (at.valid()) {
-    const UnitWalk u = at;
-    const long long row = row_of(todo.live(u.item));
-    at.next();
-    const int v0 = my_first(u), n = my_count(u);
+  for (int at = group; at < live; at += groups) {
+    const int part = part_of(todo.live(at));
+    const long long row = row_of(todo.live(at));
+    const int v0 = my_first(part), n = my_count(part);
     PolicyRow r{};
     float xt = 0.f, weight = 1.f;
     if (kMode != kRowStats && gw == 0) {  // ahead of their use
@@ -637,7 +667,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) row_kernel(T* dlogits, const T
       RowSum t = G > 1 ? fold_warps(&sums[k & 1][warp], G, lane) : fold_warp(sum);
       t.xt = xt;
       if (lane == 0) {
-        job.slots[static_cast<long long>(u.part) * job.rows + row] = t;
+        job.slots[static_cast<long long>(part) * job.rows + row] = t;
         if (kMode == kRowGrad) {
           const float c = policy_coef(args, r, weight, t);
           coef[warp] = RowCoef{finite_max(t.m), c / static_cast<float>(t.s), c, r.target};
@@ -676,7 +706,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) row_kernel(T* dlogits, const T
         if (target_here && lane == 0) elem_store(d + rc.target, value);
       }
       if (gw == G - 1) zero_vecs(reinterpret_cast<uint4*>(d) + row_vecs, job.ld / kV - row_vecs, lane, 32);
-      zero_rows(static_cast<int>(static_cast<float>(u.item + 1) * per_live));
+      zero_rows(static_cast<int>(static_cast<float>(at + 1) * per_live));
     }
   }
   if (kMode == kRowGrad) zero_rows(n_items);
@@ -692,7 +722,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) row_kernel(T* dlogits, const T
       policy_row_masked(args, row);
     } else {
       const RowSum t = job.slots[row];
-      policy_row(args, policy_row_load(args, row), row, weight, static_cast<double>(t.xt) - static_cast<double>(t.m) - log(t.s));
+      policy_row(args, policy_row_load(args, row), row, weight, logp_of(t));
     }
   }
 }
@@ -708,17 +738,15 @@ __global__ void __launch_bounds__(128) policy_rows_kernel(RowCoef* __restrict__ 
   const long long row = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
   if (row >= rows) return;
   const float w = a.weights ? a.weights[row] : 1.f;
+  const PolicyRow r = policy_row_load(a, row);
+  const RowSum t = fold_slots(slots, logits, row, rows, nslots, r.target, V, ld);
   if (w == 0.f) {
     policy_row_masked(a, row);
     if (coefs) coefs[row] = RowCoef{0.f, 0.f, 0.f, -1};
     return;
   }
-  float m;
-  double s;
-  fold_slots(slots, row, rows, nslots, &m, &s);
-  const PolicyRow r = policy_row_load(a, row);
-  const double c = policy_row(a, r, row, w, target_logp(logits, row, ld, V, r.target, m, s));
-  if (coefs) coefs[row] = RowCoef{finite_max(m), static_cast<float>(c / s), static_cast<float>(c), r.target};
+  const double c = policy_row(a, r, row, w, logp_of(t));
+  if (coefs) coefs[row] = RowCoef{finite_max(t.m), static_cast<float>(c / t.s), static_cast<float>(c), r.target};
 }
 
 // log(1 + exp(v)) without overflow.
@@ -746,16 +774,12 @@ __global__ void __launch_bounds__(kPairThreads) preference_pair_kernel(RowCoef* 
     for (int t = threadIdx.x; t < Tlen; t += kPairThreads) {
       const long long row = row0 + t;
       const float w = a.weights ? a.weights[row] : 1.f;
-      double lp = 0.0;
-      if (w != 0.f) {
-        float m;
-        double s;
-        fold_slots(slots, row, rows, nslots, &m, &s);
-        lp = target_logp(logits, row, ld, V, a.targets[row], m, s);
-        sum[side] += static_cast<double>(w) * lp;
-        // kept for the second loop, which this thread runs over the same rows
-        if (coefs) coefs[row] = RowCoef{finite_max(m), static_cast<float>(1.0 / s), 0.f, a.targets[row]};
-      }
+      const int target = a.targets[row];
+      const RowSum f = fold_slots(slots, logits, row, rows, nslots, target, V, ld);
+      const double lp = w != 0.f ? logp_of(f) : 0.0;
+      if (w != 0.f) sum[side] += static_cast<double>(w) * lp;
+      // kept for the second loop, which this thread runs over the same rows
+      if (coefs) coefs[row] = RowCoef{finite_max(f.m), static_cast<float>(1.0 / f.s), w, target};
       if (a.logps) a.logps[row] = static_cast<float>(lp);
     }
     sum[side] = warp_sum_d(sum[side]);
@@ -784,15 +808,14 @@ __global__ void __launch_bounds__(kPairThreads) preference_pair_kernel(RowCoef* 
     const long long row0 = static_cast<long long>(side * pairs + pair) * Tlen;
     for (int t = threadIdx.x; t < Tlen; t += kPairThreads) {
       const long long row = row0 + t;
-      const float w = a.weights ? a.weights[row] : 1.f;
-      if (w == 0.f) {
-        coefs[row] = RowCoef{0.f, 0.f, 0.f, -1};
+      RowCoef rcf = coefs[row];
+      if (rcf.c == 0.f) {
+        rcf = RowCoef{0.f, 0.f, 0.f, -1};
       } else {
-        RowCoef rcf = coefs[row];
-        rcf.c = static_cast<float>((side ? -slope : slope) * w);
+        rcf.c = static_cast<float>((side ? -slope : slope) * rcf.c);
         rcf.scale *= rcf.c;
-        coefs[row] = rcf;
       }
+      coefs[row] = rcf;
     }
   }
 }
@@ -880,7 +903,7 @@ bool many_rows(long long rows) { return rows >= 28LL * num_sms(); }
 int parts_of(long long rows, int V) {
   const long long want = many_rows(rows) ? std::max(2LL, (4LL * kRowWarps * num_sms() + rows - 1) / rows)
                                          : (4LL * num_sms() + rows - 1) / rows;
-  return static_cast<int>(std::max(1LL, std::min<long long>({want, 16, (V + 2047) / 2048})));
+  return static_cast<int>(std::max(1LL, std::min<long long>({want, kMaxParts, (V + 2047) / 2048})));
 }
 
 // Scratch of `rows` rows of `Vp` columns: the slot planes, then one RowCoef per
@@ -958,13 +981,13 @@ int launch_rows(void* dlogits, const void* logits, const RowJob& job, const Poli
   static bool done[64] = {};
   LLMK_TRY(allow_smem(row_kernel<T, kMode>, kRowWarps * kWarpRingBytes, done));
   const size_t smem = static_cast<size_t>(kRowWarps) * job.stages * job.sub * 16;
-  const int most = num_sms() * kMaxItems;  // rows of one launch
-  for (long long row0 = 0; row0 < job.rows; row0 += most) {
-    RowJob part = job;
-    part.row0 = static_cast<int>(row0);
-    part.row1 = static_cast<int>(std::min<long long>(job.rows, row0 + most));
-    row_kernel<T, kMode><<<std::min(part.row1 - part.row0, num_sms()), kRowThreads, smem, s>>>(
-        static_cast<T*>(dlogits), static_cast<const T*>(logits), part, a);
+  const long long units = static_cast<long long>(job.rows) * job.parts, most = static_cast<long long>(num_sms()) * kMaxItems;
+  for (long long u = 0; u < units; u += most) {
+    RowJob now = job;
+    now.unit0 = static_cast<unsigned>(u);
+    now.unit1 = static_cast<unsigned>(std::min(units, u + most));
+    row_kernel<T, kMode><<<static_cast<int>(std::min<long long>(now.unit1 - now.unit0, num_sms())), kRowThreads, smem, s>>>(
+        static_cast<T*>(dlogits), static_cast<const T*>(logits), now, a);
     count_launch();
   }
   LLMK_CUDA(cudaGetLastError());
@@ -1084,7 +1107,7 @@ __global__ void __launch_bounds__(256) logps_kernel(float* __restrict__ logps, c
   const long long row = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
   if (row >= rows) return;
   const RowSum t = sums[row];
-  logps[row] = static_cast<float>(static_cast<double>(t.xt) - static_cast<double>(t.m) - log(t.s));
+  logps[row] = static_cast<float>(logp_of(t));
 }
 
 __global__ void __launch_bounds__(1024) sum_losses_kernel(float* __restrict__ out, const float* __restrict__ x, int n, float div) {
