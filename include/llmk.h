@@ -283,12 +283,13 @@ int llmk_matmul_crossentropy_forward(float* losses, void* logits, llmk_dtype dty
  * on the log-probability of a row's target,
  *   lp = logits[row, target] - logsumexp(logits[row, :V]).
  * weights (NULL: all 1) multiplies each row's part of the loss; a row of weight
- * 0 (prompt, padding) is not read at all: its outputs are 0 and its gradient row
- * is 0 whatever it, its target or its other inputs hold. A target outside
+ * 0 (prompt, padding) takes no part: its outputs are 0 and its gradient row is 0
+ * whatever it, its target or its other inputs hold. A target outside
  * [0, V) in any other row gives NaN. dlogits (NULL: losses only) receives
  * dscale times the gradient of the summed losses, 0 on [V, Vp); it may be the
- * logits buffer itself but not overlap it otherwise. Sums run in a fixed order:
- * the same inputs give the same bits. The reference has no counterpart (its
+ * logits buffer itself but not overlap it otherwise. Up to 2^30 rows. Sums run
+ * in a fixed order: the same inputs give the same bits. A workspace serves one
+ * call at a time and may be any memory between calls. The reference has no counterpart (its
  * only loss is the cross-entropy, gpt2/cuda/cross_entropy.cu:7-32).
  *
  * llmk_policy_loss: the clipped policy loss with a KL term. With rho = exp(lp -

@@ -218,6 +218,67 @@ def test_policy_loss_special_values(cuda_dev):
         p.check()
 
 
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_policy_loss_terms_next_to_nothing(cuda_dev, dt):
+    """Two tokens share the mass, all others are where an exponential leaves fp32's normal range: the row's
+    log-probability is -log 2."""
+    for rows, V in ((3, 1000), (2, 20000)):
+        p = Policy(rows, V, V, dt, cuda_dev, seed=21, masked=0.0, ref=False, kl=0.0)
+        far = torch.arange(V, device=cuda_dev) % 9
+        p.x[:] = (-85.0 - 0.5 * far).to(dt)
+        for at in ((5, 13), (V - 3, 21), (11, V // 2 + 5)):
+            p.x[:, at[0]], p.x[:, at[1]] = 0.0, 0.0
+            p.t[:] = at[0]
+            p.old = torch.full((rows,), -0.7, device=cuda_dev)
+            p.call()
+            p.check()
+            p.x[:, at[0]], p.x[:, at[1]] = -86.0, -86.0
+
+
+def test_policy_loss_unreachable_target(cuda_dev):
+    """A target of probability 0: the KL estimate is infinite, not NaN; without a KL term the gradient vanishes."""
+    p = Policy(4, 500, 504, torch.float32, cuda_dev, seed=22, masked=0.0)
+    p.t[1] = 77
+    p.x[1, 77] = -math.inf
+    p.old[1], p.ref[1] = -3.0, -3.0
+    p.call()
+    assert p.logps[1] == -math.inf and p.kls[1] == math.inf and p.losses[1] == math.inf
+    p.call(kl_coef=0.0)
+    # rho = 0: -min(0 A, 0.8 A) is 0 for A > 0 and -0.8 A for A < 0, without a gradient either way
+    want = p.w[1].item() * max(0.0, -(1 - float(np.float32(p.lo))) * p.A[1].item())
+    assert abs(p.losses[1].item() - want) <= 2 * U * want
+    assert (p.dx[1] == 0).all() and p.kls[1] == math.inf
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_losses_of_very_many_rows(cuda_dev, grad):
+    """More rows than one launch takes on."""
+    p = Policy(350001, 7, 8, torch.bfloat16, cuda_dev, seed=23)
+    p.call(**({} if grad else dict(dlogits=None)))
+    if not grad:
+        p.dx = None
+        p.check()
+        return
+    p.check()
+    q = Preference(1, 175001, 5, 8, torch.float32, cuda_dev, seed=24, beta=1e-4)
+    q.call()
+    q.check()
+
+
+def test_losses_at_once_on_two_streams(cuda_dev):
+    """Two calls in flight, each with a workspace of its own, and masked rows all over."""
+    a, b = (Policy(700, 9001, 9008, torch.bfloat16, cuda_dev, seed=s, masked=0.6) for s in (25, 26))
+    c = Preference(3, 200, 9001, 9008, torch.float32, cuda_dev, seed=27, masked=0.6)
+    torch.cuda.synchronize()
+    s = [torch.cuda.Stream() for _ in range(3)]
+    for _ in range(5):
+        for p, st in zip((a, b, c), s):
+            p.call(stream=st)
+    torch.cuda.synchronize()
+    for p in (a, b, c):
+        p.check()
+
+
 def test_policy_gradient_by_differences(cuda_dev):
     """dlogits against the difference quotient of the summed losses, in a random direction."""
     p = Policy(40, 500, 504, torch.float32, cuda_dev, seed=10, dscale=1.0)
@@ -484,6 +545,30 @@ def test_norm_range(cuda_dev, value):
         assert norm.item() == math.inf
     else:
         assert abs(norm.item() - want) <= want * NORM + 2.0 ** -149
+
+
+def test_norm_of_nothing(cuda_dev):
+    import llmk
+    t = (llmk.Tensor * 2)(llmk.Tensor(None, None, 0, 0, 0), llmk.Tensor(None, None, 0, 1, 1))
+    norm, ws = torch.full((1,), 9.0, device=cuda_dev), torch.empty(1 << 16, dtype=torch.uint8, device=cuda_dev)
+    for name, x in (("llmk_grad_norm", 1.0), ("llmk_clip_grad_norm", 2.0)):
+        norm.fill_(9.0)
+        llmk.call(name, norm.data_ptr(), t, 2, x, ws.data_ptr(), ws.numel(), llmk.stream_ptr())
+        assert norm.item() == 0.0
+
+
+def test_clip_many_units(cuda_dev):
+    """Enough elements for a block per unit: odd sizes, an empty tensor, a start off the 16-byte grid."""
+    import llmk
+    ts = pieces([9_000_001, 0, 7, 8_191_999, 3], torch.float32, cuda_dev, 5, 1.0, 1)
+    outs = [torch.full_like(t, 9.0) for t in ts]
+    tl, norm = llmk.TensorList(ts, outs), torch.zeros(1, device=cuda_dev)
+    llmk.clip_grad_norm(norm, tl, 1.0, workspace=norm_workspace(tl, cuda_dev))
+    want = norm64(ts)
+    assert abs(norm.item() - want) <= want * NORM
+    for t, o in zip(ts, outs):
+        w = t.double() / (want + 1e-6)
+        within(o, w, w.abs() * (NORM + 5 * U) + TINY, "clipped")
 
 
 def test_norm_not_finite(cuda_dev):
