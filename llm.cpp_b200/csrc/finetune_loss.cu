@@ -756,9 +756,6 @@ __global__ void __launch_bounds__(128) policy_rows_kernel(RowCoef* __restrict__ 
   if (coefs) coefs[row] = RowCoef{finite_max(t.m), static_cast<float>(c / t.s), static_cast<float>(c), r.target};
 }
 
-// log(1 + exp(v)) without overflow.
-__device__ __forceinline__ double softplus_d(double v) { return (v > 0.0 ? v : 0.0) + log1p(exp(-fabs(v))); }
-
 // The preference loss from slots, one CTA per pair p (sequence p is the chosen
 // one, pairs + p the rejected one): L = sum_t w lp over each sequence, h =
 // beta ((L_c - R_c) - (L_r - R_r)), loss = (1 - e) log(1 + exp(-h)) + e log(1 +
@@ -793,23 +790,24 @@ __global__ void __launch_bounds__(kPairThreads) preference_pair_kernel(RowCoef* 
     if (lane == 0) red[side][warp] = sum[side];
   }
   __syncthreads();
-  double L[2] = {0.0, 0.0};
-#pragma unroll
-  for (int side = 0; side < 2; ++side)
-    for (int k = 0; k < kPairThreads / 32; ++k) L[side] += red[side][k];
-  const double beta = a.beta, e = a.smoothing;
-  const double rc = beta * (L[0] - (a.ref_logps ? static_cast<double>(a.ref_logps[pair]) : 0.0));
-  const double rr = beta * (L[1] - (a.ref_logps ? static_cast<double>(a.ref_logps[pairs + pair]) : 0.0));
+  const double L0 = warp_sum_d(red[0][lane]), L1 = warp_sum_d(red[1][lane]);
+  const double beta = a.beta, eps = a.smoothing;
+  const double rc = beta * (L0 - (a.ref_logps ? static_cast<double>(a.ref_logps[pair]) : 0.0));
+  const double rr = beta * (L1 - (a.ref_logps ? static_cast<double>(a.ref_logps[pairs + pair]) : 0.0));
   const double h = rc - rr;
+  // log(1 + exp(+-h)) and both sigmoids from exp(-|h|), which does not overflow
+  const double e = exp(-fabs(h));
   if (threadIdx.x == 0) {
-    a.losses[pair] = static_cast<float>((1.0 - e) * softplus_d(-h) + e * softplus_d(h));
+    const double t = log1p(e), up = (h > 0.0 ? h : 0.0) + t, down = (h < 0.0 ? -h : 0.0) + t;
+    a.losses[pair] = static_cast<float>(isnan(h) ? h : (1.0 - eps) * down + (eps != 0.0 ? eps * up : 0.0));
     if (a.rewards) {
       a.rewards[pair] = static_cast<float>(rc);
       a.rewards[pairs + pair] = static_cast<float>(rr);
     }
   }
   if (!coefs) return;
-  const double slope = beta * static_cast<double>(a.dscale) * (e / (1.0 + exp(-h)) - (1.0 - e) / (1.0 + exp(h)));
+  const double near = 1.0 / (1.0 + e), far = e * near;  // the sigmoids of |h| and -|h|
+  const double slope = beta * static_cast<double>(a.dscale) * (h > 0.0 ? eps * near - (1.0 - eps) * far : eps * far - (1.0 - eps) * near);
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
     const long long row0 = static_cast<long long>(side * pairs + pair) * Tlen;

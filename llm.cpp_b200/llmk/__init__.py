@@ -256,12 +256,12 @@ def _device_of(t) -> int:
     return dev
 
 
-def _check(what: str, dev: int, dtype, n: int, **tensors) -> None:
+def _check(what: str, names: str, dev: int, dtype, n: int, *tensors) -> None:
     """Each tensor (or None): of that type, contiguous with n elements, on device dev. A launch from Python is a few
     microseconds; this is kept to four tests a tensor."""
-    for t in tensors.values():
+    for t in tensors:
         if t is not None and (t.dtype is not dtype or t.numel() != n or t.get_device() != dev or not t.is_contiguous()):
-            name = next(k for k, v in tensors.items() if v is t)
+            name = names.split()[[v is t for v in tensors].index(True)]
             if t.dtype is not dtype:
                 raise TypeError(f"{what}: {name} must be {dtype}, got {t.dtype}")
             raise ValueError(f"{what}: {name} must be contiguous with {n} elements on the same device as the others, "
@@ -281,10 +281,10 @@ def policy_loss(losses, logits, targets, advantages, *, V=None, weights=None, ol
     Vp = logits.shape[-1]
     rows = logits.numel() // Vp
     dev = _device_of(logits)
-    _check("policy_loss", dev, logits.dtype, rows * Vp, logits=logits, dlogits=dlogits)
-    _check("policy_loss", dev, torch.int32, rows, targets=targets)
-    _check("policy_loss", dev, torch.float32, rows, losses=losses, advantages=advantages, weights=weights,
-           old_logps=old_logps, ref_logps=ref_logps, kls=kls, logps=logps)
+    _check("policy_loss", "logits dlogits", dev, logits.dtype, rows * Vp, logits, dlogits)
+    _check("policy_loss", "targets", dev, torch.int32, rows, targets)
+    _check("policy_loss", "losses advantages weights old_logps ref_logps kls logps", dev, torch.float32, rows, losses,
+           advantages, weights, old_logps, ref_logps, kls, logps)
     ws, ws_bytes = _ws(workspace)
     call("llmk_policy_loss", ptr(losses), ptr(kls), ptr(logps), ptr(dlogits), ptr(logits), dtype_code(logits),
          ptr(targets), ptr(weights), ptr(advantages), ptr(old_logps), ptr(ref_logps), rows, Vp if V is None else V, Vp,
@@ -306,11 +306,11 @@ def preference_loss(losses, logits, targets, *, V=None, weights=None, ref_logps=
     if pairs == 0 or rows % (2 * pairs):
         raise ValueError(f"preference_loss: {rows} rows of logits are not {pairs} pairs of sequences")
     dev = _device_of(logits)
-    _check("preference_loss", dev, logits.dtype, rows * Vp, logits=logits, dlogits=dlogits)
-    _check("preference_loss", dev, torch.int32, rows, targets=targets)
-    _check("preference_loss", dev, torch.float32, rows, weights=weights, logps=logps)
-    _check("preference_loss", dev, torch.float32, pairs, losses=losses)
-    _check("preference_loss", dev, torch.float32, 2 * pairs, ref_logps=ref_logps, rewards=rewards)
+    _check("preference_loss", "logits dlogits", dev, logits.dtype, rows * Vp, logits, dlogits)
+    _check("preference_loss", "targets", dev, torch.int32, rows, targets)
+    _check("preference_loss", "weights logps", dev, torch.float32, rows, weights, logps)
+    _check("preference_loss", "losses", dev, torch.float32, pairs, losses)
+    _check("preference_loss", "ref_logps rewards", dev, torch.float32, 2 * pairs, ref_logps, rewards)
     ws, ws_bytes = _ws(workspace)
     call("llmk_preference_loss", ptr(losses), ptr(rewards), ptr(logps), ptr(dlogits), ptr(logits), dtype_code(logits),
          ptr(targets), ptr(weights), ptr(ref_logps), pairs, rows // (2 * pairs), Vp if V is None else V, Vp, beta,
@@ -346,7 +346,7 @@ def grad_norm_workspace(tensors: TensorList) -> int:
 def grad_norm(norm, tensors: TensorList, *, scale=1.0, workspace=None, stream=None):
     """norm[0] = |scale| * the 2-norm over all tensors (llmk_grad_norm)."""
     import torch
-    _check("grad_norm", _device_of(norm), torch.float32, 1, norm=norm)
+    _check("grad_norm", "norm", _device_of(norm), torch.float32, 1, norm)
     if tensors.device != norm.get_device():
         raise ValueError("grad_norm: norm is on another device than the tensors")
     call("llmk_grad_norm", ptr(norm), tensors.array, len(tensors), scale, *_ws(workspace), stream_ptr(stream))
@@ -355,7 +355,7 @@ def grad_norm(norm, tensors: TensorList, *, scale=1.0, workspace=None, stream=No
 def clip_grad_norm(norm, tensors: TensorList, max_norm, *, workspace=None, stream=None):
     """norm[0] as grad_norm, and every tensor scaled to a global norm of at most max_norm (llmk_clip_grad_norm)."""
     import torch
-    _check("clip_grad_norm", _device_of(norm), torch.float32, 1, norm=norm)
+    _check("clip_grad_norm", "norm", _device_of(norm), torch.float32, 1, norm)
     if tensors.device != norm.get_device():
         raise ValueError("clip_grad_norm: norm is on another device than the tensors")
     call("llmk_clip_grad_norm", ptr(norm), tensors.array, len(tensors), max_norm, *_ws(workspace), stream_ptr(stream))
@@ -365,10 +365,10 @@ def adamw_clipped(params, grads, m, v, hparams, norm, max_norm, *, params_bf16=N
     """AdamW with device hyperparameters on gradients clipped by the norm in device memory (llmk_adamw_clipped)."""
     import torch
     n, dev = params.numel(), _device_of(params)
-    _check("adamw_clipped", dev, torch.float32, n, params=params, grads=grads, m=m, v=v)
-    _check("adamw_clipped", dev, torch.bfloat16, n, params_bf16=params_bf16)
-    _check("adamw_clipped", dev, torch.float32, 8, hparams=hparams)
-    _check("adamw_clipped", dev, torch.float32, 1, norm=norm)
+    _check("adamw_clipped", "params grads m v", dev, torch.float32, n, params, grads, m, v)
+    _check("adamw_clipped", "params_bf16", dev, torch.bfloat16, n, params_bf16)
+    _check("adamw_clipped", "hparams", dev, torch.float32, 8, hparams)
+    _check("adamw_clipped", "norm", dev, torch.float32, 1, norm)
     call("llmk_adamw_clipped", ptr(params), ptr(params_bf16), ptr(grads), ptr(m), ptr(v), params.numel(), ptr(hparams),
          ptr(norm), max_norm, stream_ptr(stream))
 
