@@ -909,7 +909,7 @@ bool many_rows(long long rows) { return rows >= 28LL * num_sms(); }
 int parts_of(long long rows, int V) {
   const long long want = many_rows(rows) ? std::max(2LL, (4LL * kRowWarps * num_sms() + rows - 1) / rows)
                                          : (4LL * num_sms() + rows - 1) / rows;
-  return static_cast<int>(std::max(1LL, std::min<long long>({want, kMaxParts, (V + 2047) / 2048})));
+  return static_cast<int>(std::max(1LL, std::min<long long>({want, kMaxParts, (V + 2047LL) / 2048})));
 }
 
 // Scratch of `rows` rows of `Vp` columns: the slot planes, then one RowCoef per

@@ -16,6 +16,7 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -394,25 +395,23 @@ int check_workspace(const char* what, const std::vector<Span>& spans, const void
   return LLMK_OK;
 }
 
-}  // namespace
-}  // namespace llmk
-
-using namespace llmk;
-
-extern "C" {
-
-size_t llmk_grad_norm_workspace(const llmk_tensor* tensors, int count) {
-  if (!tensors || count <= 0) return 0;
-  return workspace_of(spans_of(tensors, count));
+// The host side keeps a list of spans; a caller in C gets a status, not an
+// exception, when there is no memory for it.
+template <typename F>
+int no_throw(F f) {
+  try {
+    return f();
+  } catch (const std::bad_alloc&) {
+    return LLMK_ERR_INVALID_ARG;
+  }
 }
 
-int llmk_grad_norm(float* norm, const llmk_tensor* tensors, int count, float scale, void* workspace,
-                   size_t workspace_bytes, void* stream) {
+int grad_norm(float* norm, const llmk_tensor* tensors, int count, float scale, void* workspace, size_t workspace_bytes,
+              cudaStream_t s) {
   if (!norm || !std::isfinite(scale)) return fail(LLMK_ERR_INVALID_ARG, "grad_norm: null norm or bad scale");
   LLMK_TRY(check_tensors("grad_norm", tensors, count, false));
   const auto spans = spans_of(tensors, count);
   LLMK_TRY(check_workspace("grad_norm", spans, workspace, workspace_bytes));
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
   auto* partial = static_cast<double*>(workspace);
   const int n = launch_squares(partial, tensors, spans, s);
   LLMK_CUDA(launch_after(grad_norm_kernel, 1, kThreads, 0, s, norm, partial, n, scale));
@@ -421,13 +420,13 @@ int llmk_grad_norm(float* norm, const llmk_tensor* tensors, int count, float sca
   return LLMK_OK;
 }
 
-int llmk_clip_grad_norm(float* norm, const llmk_tensor* tensors, int count, float max_norm, void* workspace,
-                        size_t workspace_bytes, void* stream) {
+
+int clip_grad_norm(float* norm, const llmk_tensor* tensors, int count, float max_norm, void* workspace,
+                   size_t workspace_bytes, cudaStream_t s) {
   if (!norm || !(max_norm > 0.f)) return fail(LLMK_ERR_INVALID_ARG, "clip_grad_norm: null norm, or max_norm not above 0");
   LLMK_TRY(check_tensors("clip_grad_norm", tensors, count, true));
   const auto spans = spans_of(tensors, count);
   LLMK_TRY(check_workspace("clip_grad_norm", spans, workspace, workspace_bytes));
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
   auto* partial = static_cast<double*>(workspace);
   const int n = launch_squares(partial, tensors, spans, s);
   // Many units: a block for each, in order, streams faster than a fixed grid that
@@ -448,6 +447,33 @@ int llmk_clip_grad_norm(float* norm, const llmk_tensor* tensors, int count, floa
     count_launch();
   }
   return LLMK_OK;
+}
+
+}  // namespace
+}  // namespace llmk
+
+using namespace llmk;
+
+extern "C" {
+
+size_t llmk_grad_norm_workspace(const llmk_tensor* tensors, int count) {
+  if (!tensors || count <= 0) return 0;
+  size_t bytes = 0;
+  return no_throw([&] { return bytes = workspace_of(spans_of(tensors, count)), LLMK_OK; }) == LLMK_OK ? bytes : 0;
+}
+
+int llmk_grad_norm(float* norm, const llmk_tensor* tensors, int count, float scale, void* workspace,
+                   size_t workspace_bytes, void* stream) {
+  return no_throw([&] {
+    return grad_norm(norm, tensors, count, scale, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int llmk_clip_grad_norm(float* norm, const llmk_tensor* tensors, int count, float max_norm, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+  return no_throw([&] {
+    return clip_grad_norm(norm, tensors, count, max_norm, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+  });
 }
 
 }  // extern "C"
