@@ -897,18 +897,10 @@ __global__ void __launch_bounds__(kRowThreads, 1) row_gradient_kernel(T* dlogits
   ring.drain();
 }
 
-// From this many rows on, a warp works on (parts of) rows of its own where only
-// sums are wanted, and waits for no other: 8192 rows of 50257 bf16 logits 149 us
-// against 171 us by groups of warps. Below, too few units leave warps idle: 2048
-// rows 52 against 49 us, 512 rows 23 against 19 us.
-bool many_rows(long long rows) { return rows >= 28LL * num_sms(); }
-
-// Parts a row is cut into when only its sum is wanted: about four for every warp
-// of the GPU (evaluation of 8192 rows: two parts 149 us, one 158, four 159), or
-// (few rows) four for every SM, of 256 vectors of bf16 at least.
+// Parts a row is cut into when only its sum is wanted and there are few rows:
+// four units for every SM, of 256 vectors of bf16 at least.
 int parts_of(long long rows, int V) {
-  const long long want = many_rows(rows) ? std::max(2LL, (4LL * kRowWarps * num_sms() + rows - 1) / rows)
-                                         : (4LL * num_sms() + rows - 1) / rows;
+  const long long want = (4LL * num_sms() + rows - 1) / rows;
   return static_cast<int>(std::max(1LL, std::min<long long>({want, kMaxParts, (V + 2047LL) / 2048})));
 }
 
@@ -958,19 +950,14 @@ constexpr int kWarpRingBytes = 9216;
 // `keep` is asked (a unit stays in its group's rings) and it does not fit.
 bool share_out(RowJob* job, bool keep) {
   const int warp_vecs = kWarpRingBytes / 16;
-  if (!keep && many_rows(job->rows)) {
-    job->group = 1;
-    job->seg = job->vecs;
-    job->sub = std::min(div_up(job->vecs, 32) * 32, 192);
-    job->stages = std::min(kMaxStages, warp_vecs / job->sub);
-    return true;
-  }
   const long long units = static_cast<long long>(job->rows) * job->parts;
   static const int kGroups[] = {1, 2, 3, 4, 6, 8, 12, 24};  // the divisors of kRowWarps
-  // the fewest warps a unit fits, so that groups work on rows of their own and
-  // one's barriers are hidden by the others, ...
+  // the fewest warps a unit fits (or fits twice, when it only streams through:
+  // evaluation of 4096 rows 79 us, 87 us by groups it fits once), so that groups
+  // work on rows of their own and one's barriers are hidden by the others (a warp
+  // for itself, on parts of rows: 84 us, and 8192 rows of fp32 297 against 253 us), ...
   int g = 0;
-  while (kGroups[g] < kRowWarps && job->vecs > kGroups[g] * warp_vecs) ++g;
+  while (kGroups[g] < kRowWarps && job->vecs > kGroups[g] * warp_vecs * (keep ? 1 : 2)) ++g;
   if (keep && job->vecs > kGroups[g] * warp_vecs) return false;
   // ... and more when there are so few units that every one still has its group
   while (kGroups[g] < kRowWarps && units * kGroups[g + 1] <= static_cast<long long>(num_sms()) * kRowWarps && job->vecs > 32 * kGroups[g]) ++g;
@@ -1042,19 +1029,19 @@ int policy_loss(void* dlogits, const void* logits, const PolicyArgs& a, int rows
                 cudaStream_t s) {
   RowJob job = row_job<T>(a.weights, rows, V, Vp);
   job.slots = static_cast<RowSum*>(workspace);
-  if (!dlogits && !many_rows(rows)) {
+  if (!dlogits) {
     share_out(&job, false);
     return launch_rows<T, kRowEval>(nullptr, logits, job, a, s);
   }
-  if (dlogits && share_out(&job, true)) return launch_rows<T, kRowGrad>(dlogits, logits, job, a, s);
+  if (share_out(&job, true)) return launch_rows<T, kRowGrad>(dlogits, logits, job, a, s);
   RowSum* slots = job.slots;
-  auto* coefs = dlogits ? reinterpret_cast<RowCoef*>(static_cast<char*>(workspace) + slots_bytes(rows, Vp)) : nullptr;
+  auto* coefs = reinterpret_cast<RowCoef*>(static_cast<char*>(workspace) + slots_bytes(rows, Vp));
   int nslots = 0;
   LLMK_TRY(launch_slots<T>(slots, &nslots, logits, a.weights, rows, V, Vp, s));
   LLMK_CUDA(launch_after(policy_rows_kernel<T>, div_up(rows, 128), 128, 0, s, coefs, slots,
                          static_cast<const T*>(logits), a, rows, V, Vp, nslots));
   count_launch();
-  return dlogits ? launch_gradient<T>(dlogits, logits, coefs, rows, V, Vp, s) : LLMK_OK;
+  return launch_gradient<T>(dlogits, logits, coefs, rows, V, Vp, s);
 }
 
 template <typename T>
