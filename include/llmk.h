@@ -287,7 +287,8 @@ int llmk_matmul_crossentropy_forward(float* losses, void* logits, llmk_dtype dty
  * whatever it, its target or its other inputs hold. A target outside
  * [0, V) in any other row gives NaN. dlogits (NULL: losses only) receives
  * dscale times the gradient of the summed losses, 0 on [V, Vp); it may be the
- * logits buffer itself but not overlap it otherwise. Up to 2^30 rows. Sums run
+ * logits buffer itself but not overlap it otherwise. The per-row and per-sequence
+ * outputs may be buffers of their inputs of the same size. Up to 2^30 rows. Sums run
  * in a fixed order: the same inputs give the same bits. A workspace serves one
  * call at a time and may be any memory between calls. The reference has no counterpart (its
  * only loss is the cross-entropy, gpt2/cuda/cross_entropy.cu:7-32).

@@ -771,6 +771,8 @@ __global__ void __launch_bounds__(kPairThreads) preference_pair_kernel(RowCoef* 
   grid_wait();
   const int pair = blockIdx.x, rows = 2 * pairs * Tlen;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // before the barrier that the outputs come after: rewards may be ref_logps
+  const float ref0 = a.ref_logps ? a.ref_logps[pair] : 0.f, ref1 = a.ref_logps ? a.ref_logps[pairs + pair] : 0.f;
   double sum[2] = {0.0, 0.0};
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
@@ -792,8 +794,7 @@ __global__ void __launch_bounds__(kPairThreads) preference_pair_kernel(RowCoef* 
   __syncthreads();
   const double L0 = warp_sum_d(red[0][lane]), L1 = warp_sum_d(red[1][lane]);
   const double beta = a.beta, eps = a.smoothing;
-  const double rc = beta * (L0 - (a.ref_logps ? static_cast<double>(a.ref_logps[pair]) : 0.0));
-  const double rr = beta * (L1 - (a.ref_logps ? static_cast<double>(a.ref_logps[pairs + pair]) : 0.0));
+  const double rc = beta * (L0 - static_cast<double>(ref0)), rr = beta * (L1 - static_cast<double>(ref1));
   const double h = rc - rr;
   // log(1 + exp(+-h)) and both sigmoids from exp(-|h|), which does not overflow
   const double e = exp(-fabs(h));

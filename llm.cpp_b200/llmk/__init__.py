@@ -278,8 +278,7 @@ def policy_loss(losses, logits, targets, advantages, *, V=None, weights=None, ol
                 stream=None):
     """Clipped policy loss over logits (..., Vp), and its gradient when dlogits is given (llmk_policy_loss)."""
     import torch
-    Vp = logits.shape[-1]
-    rows = logits.numel() // Vp
+    Vp, rows = logits.shape[-1], targets.numel()
     dev = _device_of(logits)
     _check("policy_loss", "logits dlogits", dev, logits.dtype, rows * Vp, logits, dlogits)
     _check("policy_loss", "targets", dev, torch.int32, rows, targets)
@@ -301,10 +300,9 @@ def preference_loss(losses, logits, targets, *, V=None, weights=None, ref_logps=
     """Preference loss over losses.numel() pairs of sequences of logits (..., Vp), the preferred ones first, and its
     gradient when dlogits is given (llmk_preference_loss)."""
     import torch
-    Vp, pairs = logits.shape[-1], losses.numel()
-    rows = logits.numel() // Vp
+    Vp, rows, pairs = logits.shape[-1], targets.numel(), losses.numel()
     if pairs == 0 or rows % (2 * pairs):
-        raise ValueError(f"preference_loss: {rows} rows of logits are not {pairs} pairs of sequences")
+        raise ValueError(f"preference_loss: {rows} rows are not {pairs} pairs of sequences")
     dev = _device_of(logits)
     _check("preference_loss", "logits dlogits", dev, logits.dtype, rows * Vp, logits, dlogits)
     _check("preference_loss", "targets", dev, torch.int32, rows, targets)

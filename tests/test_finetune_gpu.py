@@ -446,6 +446,23 @@ def test_losses_repeat_bit_for_bit_on_another_stream_and_in_a_graph(cuda_dev, wh
     del graph
 
 
+@pytest.mark.parametrize("V,Vp", [(101, 104), (50257, 50304), (131072, 131080)])
+def test_per_row_outputs_over_inputs(cuda_dev, V, Vp):
+    """An output may take the place of an input of its size: every row and pair reads its own before it writes."""
+    p = Policy(70, V, Vp, torch.bfloat16, cuda_dev, seed=21)
+    p.call()
+    want = [t.clone() for t in (p.losses, p.kls, p.logps, p.dx)]
+    p.losses, kls, logps = p.w, p.ref, p.old
+    p.call(kls=kls, logps=logps)
+    assert all(torch.equal(a, b) for a, b in zip(want, (p.losses, kls, logps, p.dx)))
+    q = Preference(40, 3, V, Vp, torch.bfloat16, cuda_dev, seed=22)
+    q.call()
+    want = [t.clone() for t in (q.losses, q.rewards, q.logps, q.dx)]
+    rewards, logps = q.ref, q.w
+    q.call(rewards=rewards, logps=logps)
+    assert all(torch.equal(a, b) for a, b in zip(want, (q.losses, rewards, logps, q.dx)))
+
+
 def test_two_graphs_share_a_workspace(cuda_dev):
     a, b = Policy(50, 3001, 3008, torch.float32, cuda_dev, seed=13), Preference(2, 20, 3001, 3008, torch.float32, cuda_dev, seed=14)
     ws = a.ws if a.ws.numel() > b.ws.numel() else b.ws
@@ -665,6 +682,8 @@ def test_wrappers_refuse_wrong_tensors(cuda_dev):
     for kw in (dict(ref_logps=q.ref[:3]), dict(rewards=q.losses), dict(logits=q.x[:11])):
         with pytest.raises((TypeError, ValueError)):
             q.call(**kw)
+    with pytest.raises(llmk.LlmkError):
+        p.call(logits=p.x[:, :0], dlogits=None, V=None)  # no vocabulary
     with pytest.raises(llmk.LlmkError) as e:
         p.call(workspace=p.ws[:16])
     assert e.value.code == 5
