@@ -766,39 +766,39 @@ __global__ void __launch_bounds__(kPairThreads) preference_pair_kernel(RowCoef* 
                                                                        RowSum* __restrict__ slots,
                                                                        const T* __restrict__ logits, PreferenceArgs a,
                                                                        int pairs, int Tlen, int V, int ld, int nslots) {
-  __shared__ double red[2][kPairThreads / 32];
+  constexpr int kSide = kPairThreads / 2;  // threads of a sequence
+  __shared__ double red[2][kSide / 32];
   grid_release();
   grid_wait();
   const int pair = blockIdx.x, rows = 2 * pairs * Tlen;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, side = threadIdx.x / kSide, first = threadIdx.x % kSide;
+  const long long row0 = static_cast<long long>(side * pairs + pair) * Tlen;
   // before the barrier that the outputs come after: rewards may be ref_logps
   const float ref0 = a.ref_logps ? a.ref_logps[pair] : 0.f, ref1 = a.ref_logps ? a.ref_logps[pairs + pair] : 0.f;
-  double sum[2] = {0.0, 0.0};
-#pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    const long long row0 = static_cast<long long>(side * pairs + pair) * Tlen;
-    for (int t = threadIdx.x; t < Tlen; t += kPairThreads) {
-      const long long row = row0 + t;
-      const float w = a.weights ? a.weights[row] : 1.f;
-      const int target = a.targets[row];
-      const RowSum f = fold_slots(slots, logits, row, rows, nslots, target, V, ld);
-      const double lp = w != 0.f ? logp_of(f) : 0.0;
-      if (w != 0.f) sum[side] += static_cast<double>(w) * lp;
-      // kept for the second loop, which this thread runs over the same rows
-      if (coefs) coefs[row] = RowCoef{finite_max(f.m), static_cast<float>(1.0 / f.s), w, target};
-      if (a.logps) a.logps[row] = static_cast<float>(lp);
-    }
-    sum[side] = warp_sum_d(sum[side]);
-    if (lane == 0) red[side][warp] = sum[side];
+  double sum = 0.0;
+  RowCoef mine{0.f, 0.f, 0.f, -1};  // of the thread's first row; the others' wait in memory
+  for (int t = first; t < Tlen; t += kSide) {
+    const long long row = row0 + t;
+    const float w = a.weights ? a.weights[row] : 1.f;
+    const int target = a.targets[row];
+    const RowSum f = fold_slots(slots, logits, row, rows, nslots, target, V, ld);
+    const double lp = w != 0.f ? logp_of(f) : 0.0;
+    if (w != 0.f) sum += static_cast<double>(w) * lp;
+    const RowCoef c{finite_max(f.m), static_cast<float>(1.0 / f.s), w, target};
+    if (t == first) mine = c;
+    else if (coefs) coefs[row] = c;
+    if (a.logps) a.logps[row] = static_cast<float>(lp);
   }
+  sum = warp_sum_d(sum);
+  if (lane == 0) red[side][first / 32] = sum;
   __syncthreads();
-  const double L0 = warp_sum_d(red[0][lane]), L1 = warp_sum_d(red[1][lane]);
+  const double L0 = warp_sum_d(lane < kSide / 32 ? red[0][lane] : 0.0), L1 = warp_sum_d(lane < kSide / 32 ? red[1][lane] : 0.0);
   const double beta = a.beta, eps = a.smoothing;
   const double rc = beta * (L0 - static_cast<double>(ref0)), rr = beta * (L1 - static_cast<double>(ref1));
   const double h = rc - rr;
   // log(1 + exp(+-h)) and both sigmoids from exp(-|h|), which does not overflow
   const double e = exp(-fabs(h));
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == kPairThreads - 1) {  // of a warp that seldom has rows
     const double t = log1p(e), up = (h > 0.0 ? h : 0.0) + t, down = (h < 0.0 ? -h : 0.0) + t;
     a.losses[pair] = static_cast<float>(isnan(h) ? h : (1.0 - eps) * down + (eps != 0.0 ? eps * up : 0.0));
     if (a.rewards) {
@@ -809,20 +809,15 @@ __global__ void __launch_bounds__(kPairThreads) preference_pair_kernel(RowCoef* 
   if (!coefs) return;
   const double near = 1.0 / (1.0 + e), far = e * near;  // the sigmoids of |h| and -|h|
   const double slope = beta * static_cast<double>(a.dscale) * (h > 0.0 ? eps * near - (1.0 - eps) * far : eps * far - (1.0 - eps) * near);
-#pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    const long long row0 = static_cast<long long>(side * pairs + pair) * Tlen;
-    for (int t = threadIdx.x; t < Tlen; t += kPairThreads) {
-      const long long row = row0 + t;
-      RowCoef rcf = coefs[row];
-      if (rcf.c == 0.f) {
-        rcf = RowCoef{0.f, 0.f, 0.f, -1};
-      } else {
-        rcf.c = static_cast<float>((side ? -slope : slope) * rcf.c);
-        rcf.scale *= rcf.c;
-      }
-      coefs[row] = rcf;
+  for (int t = first; t < Tlen; t += kSide) {
+    RowCoef c = t == first ? mine : coefs[row0 + t];
+    if (c.c == 0.f) {
+      c = RowCoef{0.f, 0.f, 0.f, -1};
+    } else {
+      c.c = static_cast<float>((side ? -slope : slope) * c.c);
+      c.scale *= c.c;
     }
+    coefs[row0 + t] = c;
   }
 }
 
