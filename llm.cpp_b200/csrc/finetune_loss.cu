@@ -69,14 +69,10 @@ __device__ __forceinline__ double warp_sum_d(double v) {
 // sum 0 (or NaN, when it holds one), not exp(-inf + inf).
 __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.f : m; }
 
-// A row's sum from its slots, and its target's logit (NaN for a target outside
-// [0, V)). The loads do not wait for one another but for the logit, which needs
-// the target.
+// A row's sum from its slots, given its target's logit (NaN for a target outside
+// [0, V)). The loads do not wait for one another.
 constexpr int kMaxParts = 16;
-template <typename T>
-__device__ __forceinline__ RowSum fold_slots(const RowSum* __restrict__ slots, const T* logits, long long row, int rows,
-                                             int nslots, int target, int V, int ld) {
-  const float xt = target >= 0 && target < V ? elem_to_float(logits[row * ld + target]) : NAN;
+__device__ __forceinline__ RowSum fold_slots(const RowSum* __restrict__ slots, long long row, int rows, int nslots, float xt) {
   if (nslots == 1) {
     RowSum t = slots[row];
     t.xt = xt;
@@ -746,7 +742,8 @@ __global__ void __launch_bounds__(128) policy_rows_kernel(RowCoef* __restrict__ 
   if (row >= rows) return;
   const float w = a.weights ? a.weights[row] : 1.f;
   const PolicyRow r = policy_row_load(a, row);
-  const RowSum t = fold_slots(slots, logits, row, rows, nslots, r.target, V, ld);
+  const RowSum t = fold_slots(slots, row, rows, nslots,
+                              r.target >= 0 && r.target < V ? elem_to_float(logits[row * ld + r.target]) : NAN);
   if (w == 0.f) {
     policy_row_masked(a, row);
     if (coefs) coefs[row] = RowCoef{0.f, 0.f, 0.f, -1};
@@ -760,8 +757,11 @@ __global__ void __launch_bounds__(128) policy_rows_kernel(RowCoef* __restrict__ 
 // one, pairs + p the rejected one): L = sum_t w lp over each sequence, h =
 // beta ((L_c - R_c) - (L_r - R_r)), loss = (1 - e) log(1 + exp(-h)) + e log(1 +
 // exp(h)). The sums run in a fixed order in 64 bits.
+// kEarly: the kernel before only writes slots and began after all before it (a
+// plain launch), so that this one may read its other inputs while that one runs
+// (8 pairs of 1024: 602 -> 598 us, 2 of 64: 21.9 -> 20.8 us).
 constexpr int kPairThreads = 1024;
-template <typename T>
+template <typename T, bool kEarly>
 __global__ void __launch_bounds__(kPairThreads) preference_pair_kernel(RowCoef* __restrict__ coefs,
                                                                        RowSum* __restrict__ slots,
                                                                        const T* __restrict__ logits, PreferenceArgs a,
@@ -769,19 +769,27 @@ __global__ void __launch_bounds__(kPairThreads) preference_pair_kernel(RowCoef* 
   constexpr int kSide = kPairThreads / 2;  // threads of a sequence
   __shared__ double red[2][kSide / 32];
   grid_release();
-  grid_wait();
   const int pair = blockIdx.x, rows = 2 * pairs * Tlen;
   const int lane = threadIdx.x & 31, side = threadIdx.x / kSide, first = threadIdx.x % kSide;
   const long long row0 = static_cast<long long>(side * pairs + pair) * Tlen;
+  float w = 0.f, xt = NAN;
+  int target = -1;
+  auto fetch = [&](int t) {
+    if (t >= Tlen) return;
+    w = a.weights ? a.weights[row0 + t] : 1.f;
+    target = a.targets[row0 + t];
+    xt = target >= 0 && target < V ? elem_to_float(logits[(row0 + t) * ld + target]) : NAN;
+  };
+  if (kEarly) fetch(first);
+  grid_wait();
   // before the barrier that the outputs come after: rewards may be ref_logps
   const float ref0 = a.ref_logps ? a.ref_logps[pair] : 0.f, ref1 = a.ref_logps ? a.ref_logps[pairs + pair] : 0.f;
   double sum = 0.0;
   RowCoef mine{0.f, 0.f, 0.f, -1};  // of the thread's first row; the others' wait in memory
   for (int t = first; t < Tlen; t += kSide) {
     const long long row = row0 + t;
-    const float w = a.weights ? a.weights[row] : 1.f;
-    const int target = a.targets[row];
-    const RowSum f = fold_slots(slots, logits, row, rows, nslots, target, V, ld);
+    if (!kEarly || t != first) fetch(t);
+    const RowSum f = fold_slots(slots, row, rows, nslots, xt);
     const double lp = w != 0.f ? logp_of(f) : 0.0;
     if (w != 0.f) sum += static_cast<double>(w) * lp;
     const RowCoef c{finite_max(f.m), static_cast<float>(1.0 / f.s), w, target};
@@ -1048,7 +1056,7 @@ int preference_loss(void* dlogits, const void* logits, const PreferenceArgs& a, 
   auto* coefs = dlogits ? reinterpret_cast<RowCoef*>(static_cast<char*>(workspace) + slots_bytes(rows, Vp)) : nullptr;
   int nslots = 0;
   LLMK_TRY(launch_slots<T>(slots, &nslots, logits, a.weights, rows, V, Vp, s));
-  LLMK_CUDA(launch_after(preference_pair_kernel<T>, pairs, kPairThreads, 0, s, coefs, slots,
+  LLMK_CUDA(launch_after(preference_pair_kernel<T, true>, pairs, kPairThreads, 0, s, coefs, slots,
                          static_cast<const T*>(logits), a, pairs, Tlen, V, Vp, nslots));
   count_launch();
   return dlogits ? launch_gradient<T>(dlogits, logits, coefs, rows, V, Vp, s) : LLMK_OK;
@@ -1147,7 +1155,7 @@ int preference_finish_t(void* logits, const float2* stats, const PreferenceArgs&
   const Scratch w = split(scratch, rows);
   LLMK_TRY(launch_fold<T>(w.sums, stats, logits, a.targets, rows, V, ld, s));
   RowCoef* coefs = backward ? w.coefs : nullptr;
-  LLMK_CUDA(launch_after(preference_pair_kernel<T>, pairs, kPairThreads, 0, s, coefs, w.sums,
+  LLMK_CUDA(launch_after(preference_pair_kernel<T, false>, pairs, kPairThreads, 0, s, coefs, w.sums,
                          static_cast<const T*>(logits), a, pairs, Tlen, V, ld, 1));
   count_launch();
   return backward ? launch_gradient<T>(logits, logits, w.coefs, rows, V, ld, s) : LLMK_OK;
