@@ -199,14 +199,15 @@ def ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
 
 
-def stream_ptr(stream=None) -> int | None:
-    import torch
+def stream_ptr(stream=None, device=None) -> int | None:
+    """Handle of a torch stream, or of the current one (of the current device, unless given)."""
     if stream is not None:
         return stream.cuda_stream
+    torch = _torch()
     raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # 0.2 us; the stream object below takes 3
     if raw is not None:
-        return raw(torch.cuda.current_device())
-    return torch.cuda.current_stream().cuda_stream
+        return raw(torch.cuda.current_device() if device is None else device)
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 def dtype_code(t) -> int:
@@ -243,29 +244,49 @@ def gemm(D, A, B, *, a_trans=False, b_trans=False, math=MATH_BF16, bias=None, re
          B.stride(0), math, M, N, K, C.byref(ep), ptr(workspace), ws_bytes, stream_ptr(stream))
 
 
-def _ws(workspace) -> tuple[int | None, int]:
-    return (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
+_TORCH = None
 
 
-def _device_of(t) -> int:
-    """Device index of t, which has to be the current CUDA device (the library launches there)."""
-    import torch
-    dev = t.get_device()
-    if dev < 0 or dev != torch.cuda.current_device():
+def _torch():
+    global _TORCH
+    if _TORCH is None:
+        import torch
+        _TORCH = torch
+    return _TORCH
+
+
+def _place(t, stream) -> tuple[int, int | None]:
+    """Device index of t, which has to be the current CUDA device (the library launches there), and the stream."""
+    cuda, dev = _torch().cuda, t.get_device()
+    if dev < 0 or dev != cuda.current_device():
         raise ValueError(f"expected a tensor on the current CUDA device, got one on {t.device}")
-    return dev
+    return dev, stream_ptr(stream, dev)
 
 
-def _check(what: str, names: str, dev: int, dtype, n: int, *tensors) -> None:
-    """Each tensor (or None): of that type, contiguous with n elements, on device dev. A launch from Python is a few
-    microseconds; this is kept to four tests a tensor."""
+def _ptrs(what: str, names: str, dev: int, dtype, n: int, *tensors) -> list[int | None]:
+    """Addresses of tensors (or None), each of that type, contiguous with n elements, on device dev. A launch from Python
+    is a few microseconds; this is kept to five calls a tensor."""
+    out = []
     for t in tensors:
-        if t is not None and (t.dtype is not dtype or t.numel() != n or t.get_device() != dev or not t.is_contiguous()):
-            name = names.split()[[v is t for v in tensors].index(True)]
-            if t.dtype is not dtype:
-                raise TypeError(f"{what}: {name} must be {dtype}, got {t.dtype}")
-            raise ValueError(f"{what}: {name} must be contiguous with {n} elements on the same device as the others, "
-                             f"got {tuple(t.shape)} on {t.device}")
+        if t is None:
+            out.append(None)
+        elif t.dtype is dtype and t.numel() == n and t.get_device() == dev and t.is_contiguous():
+            out.append(t.data_ptr())
+        elif t.dtype is not dtype:
+            raise TypeError(f"{what}: {names.split()[len(out)]} must be {dtype}, got {t.dtype}")
+        else:
+            raise ValueError(f"{what}: {names.split()[len(out)]} must be contiguous with {n} elements on the same device as "
+                             f"the others, got {tuple(t.shape)} on {t.device}")
+    return out
+
+
+def _ws(what: str, workspace, dev: int) -> tuple[int | None, int]:
+    if workspace is None:
+        return None, 0
+    if workspace.get_device() != dev or not workspace.is_contiguous():
+        raise ValueError(f"{what}: workspace must be contiguous on the same device as the tensors, got one on "
+                         f"{workspace.device}")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
 def policy_loss_workspace(rows: int, Vp: int) -> int:
@@ -277,17 +298,16 @@ def policy_loss(losses, logits, targets, advantages, *, V=None, weights=None, ol
                 logps=None, dlogits=None, clip_low=0.2, clip_high=0.2, kl_coef=0.0, dscale=1.0, workspace=None,
                 stream=None):
     """Clipped policy loss over logits (..., Vp), and its gradient when dlogits is given (llmk_policy_loss)."""
-    import torch
+    what, torch = "policy_loss", _torch()
     Vp, rows = logits.shape[-1], targets.numel()
-    dev = _device_of(logits)
-    _check("policy_loss", "logits dlogits", dev, logits.dtype, rows * Vp, logits, dlogits)
-    _check("policy_loss", "targets", dev, torch.int32, rows, targets)
-    _check("policy_loss", "losses advantages weights old_logps ref_logps kls logps", dev, torch.float32, rows, losses,
-           advantages, weights, old_logps, ref_logps, kls, logps)
-    ws, ws_bytes = _ws(workspace)
-    call("llmk_policy_loss", ptr(losses), ptr(kls), ptr(logps), ptr(dlogits), ptr(logits), dtype_code(logits),
-         ptr(targets), ptr(weights), ptr(advantages), ptr(old_logps), ptr(ref_logps), rows, Vp if V is None else V, Vp,
-         clip_low, clip_high, kl_coef, dscale, ws, ws_bytes, stream_ptr(stream))
+    dev, s = _place(logits, stream)
+    x, dx = _ptrs(what, "logits dlogits", dev, logits.dtype, rows * Vp, logits, dlogits)
+    tgt, = _ptrs(what, "targets", dev, torch.int32, rows, targets)
+    loss, kl, lp, w, adv, old, ref = _ptrs(what, "losses kls logps weights advantages old_logps ref_logps", dev,
+                                           torch.float32, rows, losses, kls, logps, weights, advantages, old_logps,
+                                           ref_logps)
+    call("llmk_policy_loss", loss, kl, lp, dx, x, dtype_code(logits), tgt, w, adv, old, ref, rows, Vp if V is None else V,
+         Vp, clip_low, clip_high, kl_coef, dscale, *_ws(what, workspace, dev), s)
 
 
 def preference_loss_workspace(pairs: int, T: int, Vp: int) -> int:
@@ -299,20 +319,19 @@ def preference_loss(losses, logits, targets, *, V=None, weights=None, ref_logps=
                     dlogits=None, beta=0.1, label_smoothing=0.0, dscale=1.0, workspace=None, stream=None):
     """Preference loss over losses.numel() pairs of sequences of logits (..., Vp), the preferred ones first, and its
     gradient when dlogits is given (llmk_preference_loss)."""
-    import torch
+    what, torch = "preference_loss", _torch()
     Vp, rows, pairs = logits.shape[-1], targets.numel(), losses.numel()
     if pairs == 0 or rows % (2 * pairs):
         raise ValueError(f"preference_loss: {rows} rows are not {pairs} pairs of sequences")
-    dev = _device_of(logits)
-    _check("preference_loss", "logits dlogits", dev, logits.dtype, rows * Vp, logits, dlogits)
-    _check("preference_loss", "targets", dev, torch.int32, rows, targets)
-    _check("preference_loss", "weights logps", dev, torch.float32, rows, weights, logps)
-    _check("preference_loss", "losses", dev, torch.float32, pairs, losses)
-    _check("preference_loss", "ref_logps rewards", dev, torch.float32, 2 * pairs, ref_logps, rewards)
-    ws, ws_bytes = _ws(workspace)
-    call("llmk_preference_loss", ptr(losses), ptr(rewards), ptr(logps), ptr(dlogits), ptr(logits), dtype_code(logits),
-         ptr(targets), ptr(weights), ptr(ref_logps), pairs, rows // (2 * pairs), Vp if V is None else V, Vp, beta,
-         label_smoothing, dscale, ws, ws_bytes, stream_ptr(stream))
+    dev, s = _place(logits, stream)
+    f32 = torch.float32
+    x, dx = _ptrs(what, "logits dlogits", dev, logits.dtype, rows * Vp, logits, dlogits)
+    tgt, = _ptrs(what, "targets", dev, torch.int32, rows, targets)
+    w, lp = _ptrs(what, "weights logps", dev, f32, rows, weights, logps)
+    loss, = _ptrs(what, "losses", dev, f32, pairs, losses)
+    ref, rew = _ptrs(what, "ref_logps rewards", dev, f32, 2 * pairs, ref_logps, rewards)
+    call("llmk_preference_loss", loss, rew, lp, dx, x, dtype_code(logits), tgt, w, ref, pairs, rows // (2 * pairs),
+         Vp if V is None else V, Vp, beta, label_smoothing, dscale, *_ws(what, workspace, dev), s)
 
 
 class TensorList:
@@ -326,7 +345,7 @@ class TensorList:
             raise ValueError("TensorList: outs must match tensors")
         if not all(t.is_contiguous() for t in self.tensors + self.outs):
             raise ValueError("TensorList: tensors must be contiguous")
-        self.device = _device_of(self.tensors[0]) if self.tensors else -1
+        self.device = _place(self.tensors[0], None)[0] if self.tensors else -1
         if any(t.get_device() != self.device for t in self.tensors + self.outs):
             raise ValueError("TensorList: all tensors must be on one device")
         self.array = (Tensor * len(self.tensors))(*[Tensor(a.data_ptr(), b.data_ptr(), a.numel(), dtype_code(a),
@@ -341,34 +360,35 @@ def grad_norm_workspace(tensors: TensorList) -> int:
     return lib().llmk_grad_norm_workspace(tensors.array, len(tensors))
 
 
+def _norm_args(what: str, norm, tensors: TensorList, workspace, stream) -> tuple:
+    dev, s = _place(norm, stream)
+    out, = _ptrs(what, "norm", dev, _torch().float32, 1, norm)
+    if tensors.device != dev:
+        raise ValueError(f"{what}: norm is on another device than the tensors")
+    return out, *_ws(what, workspace, dev), s
+
+
 def grad_norm(norm, tensors: TensorList, *, scale=1.0, workspace=None, stream=None):
     """norm[0] = |scale| * the 2-norm over all tensors (llmk_grad_norm)."""
-    import torch
-    _check("grad_norm", "norm", _device_of(norm), torch.float32, 1, norm)
-    if tensors.device != norm.get_device():
-        raise ValueError("grad_norm: norm is on another device than the tensors")
-    call("llmk_grad_norm", ptr(norm), tensors.array, len(tensors), scale, *_ws(workspace), stream_ptr(stream))
+    out, ws, ws_bytes, s = _norm_args("grad_norm", norm, tensors, workspace, stream)
+    call("llmk_grad_norm", out, tensors.array, len(tensors), scale, ws, ws_bytes, s)
 
 
 def clip_grad_norm(norm, tensors: TensorList, max_norm, *, workspace=None, stream=None):
     """norm[0] as grad_norm, and every tensor scaled to a global norm of at most max_norm (llmk_clip_grad_norm)."""
-    import torch
-    _check("clip_grad_norm", "norm", _device_of(norm), torch.float32, 1, norm)
-    if tensors.device != norm.get_device():
-        raise ValueError("clip_grad_norm: norm is on another device than the tensors")
-    call("llmk_clip_grad_norm", ptr(norm), tensors.array, len(tensors), max_norm, *_ws(workspace), stream_ptr(stream))
+    out, ws, ws_bytes, s = _norm_args("clip_grad_norm", norm, tensors, workspace, stream)
+    call("llmk_clip_grad_norm", out, tensors.array, len(tensors), max_norm, ws, ws_bytes, s)
 
 
 def adamw_clipped(params, grads, m, v, hparams, norm, max_norm, *, params_bf16=None, stream=None):
     """AdamW with device hyperparameters on gradients clipped by the norm in device memory (llmk_adamw_clipped)."""
-    import torch
-    n, dev = params.numel(), _device_of(params)
-    _check("adamw_clipped", "params grads m v", dev, torch.float32, n, params, grads, m, v)
-    _check("adamw_clipped", "params_bf16", dev, torch.bfloat16, n, params_bf16)
-    _check("adamw_clipped", "hparams", dev, torch.float32, 8, hparams)
-    _check("adamw_clipped", "norm", dev, torch.float32, 1, norm)
-    call("llmk_adamw_clipped", ptr(params), ptr(params_bf16), ptr(grads), ptr(m), ptr(v), params.numel(), ptr(hparams),
-         ptr(norm), max_norm, stream_ptr(stream))
+    what, torch = "adamw_clipped", _torch()
+    n, (dev, s) = params.numel(), _place(params, stream)
+    p, g, mm, vv = _ptrs(what, "params grads m v", dev, torch.float32, n, params, grads, m, v)
+    pb, = _ptrs(what, "params_bf16", dev, torch.bfloat16, n, params_bf16)
+    hp, = _ptrs(what, "hparams", dev, torch.float32, 8, hparams)
+    nm, = _ptrs(what, "norm", dev, torch.float32, 1, norm)
+    call("llmk_adamw_clipped", p, pb, g, mm, vv, n, hp, nm, max_norm, s)
 
 
 class GPT2:

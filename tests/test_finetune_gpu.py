@@ -682,6 +682,14 @@ def test_wrappers_refuse_wrong_tensors(cuda_dev):
     for kw in (dict(ref_logps=q.ref[:3]), dict(rewards=q.losses), dict(logits=q.x[:11])):
         with pytest.raises((TypeError, ValueError)):
             q.call(**kw)
+    for c in (p, q):  # a workspace that the GPU cannot reach, or does not own whole
+        for ws in (c.ws.cpu(), c.ws.repeat(2)[::2]):
+            with pytest.raises(ValueError):
+                c.call(workspace=ws)
+    tl, norm = llmk.TensorList([p.w]), torch.zeros(1, device=cuda_dev)
+    for call in (lambda ws: llmk.grad_norm(norm, tl, workspace=ws), lambda ws: llmk.clip_grad_norm(norm, tl, 1.0, workspace=ws)):
+        with pytest.raises(ValueError):
+            call(norm_workspace(tl, "cpu"))
     with pytest.raises(llmk.LlmkError):
         p.call(logits=p.x[:, :0], dlogits=None, V=None)  # no vocabulary
     with pytest.raises(llmk.LlmkError) as e:
