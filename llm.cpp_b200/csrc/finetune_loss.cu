@@ -15,8 +15,9 @@
 // preference loss needs the sums over whole sequences before the first gradient:
 // row_kernel leaves each row's (max, sum), preference_pair_kernel forms the
 // losses and every row's coefficient, and row_gradient_kernel streams the logits
-// a second time: 8 pairs of 1024 positions in 600 us, 5.5 TB/s of 3.30 GB. Rows
-// too long for shared memory take that second way for the policy loss too.
+// a second time: 8 pairs of 1024 positions in 598 us, 5.5 TB/s of 3.30 GB. A few
+// long rows take that second way for the policy loss too. Of two variants that a
+// comment compares, both were measured with the rest of the kernel as it was then.
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -528,7 +529,8 @@ struct RowList {
   __device__ __forceinline__ int dead(int i, int n) const { return items[n - 1 - i]; }
 };
 
-enum RowMode { kRowGrad, kRowEval, kRowStats };
+// kRowLong: kRowGrad for rows that do not fit their group's rings.
+enum RowMode { kRowGrad, kRowLong, kRowEval, kRowStats };
 
 // How row_kernel shares the work out. A unit is a row, or (kRowStats) one of
 // `parts` parts of it, of `vecs` vectors; a launch covers units [unit0, unit1) of
@@ -551,12 +553,16 @@ struct RowJob {
 // joins the sums and forms the row's coefficient; in kRowGrad the chunks stay in
 // shared memory until pass B has written the gradient from them, so the logits
 // are read from memory once, and each chunk's place is then refilled with the
-// group's next row. Masked rows take no chunk. Each unit's (max, sum) goes to its
+// group's next row. In kRowLong the first chunks give up their places in pass A
+// and come again, from L2 (148 rows are on their way), after the ones that stayed:
+// 4096 rows of 131072, half live, in 312 us; by two kernels over all rows 406.
+// Masked rows take no chunk. Each unit's (max, sum) goes to its
 // slot, planes of `rows`. A wait that is given up (the device status says so)
 // ends the work, not the barriers: the group's warps still meet.
 template <typename T, int kMode>
 __global__ void __launch_bounds__(kRowThreads, 1) row_kernel(T* dlogits, const T* logits, RowJob job, PolicyArgs args) {
   constexpr int kV = vec_elems<T>();
+  constexpr bool kGrad = kMode == kRowGrad || kMode == kRowLong;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t bars[kRowWarps * kMaxStages];
   __shared__ WarpSum sums[2][kRowWarps];
@@ -600,21 +606,28 @@ __global__ void __launch_bounds__(kRowThreads, 1) row_kernel(T* dlogits, const T
     return max(0, min(job.seg, min(job.vecs, row_vecs - part * job.vecs) - gw * job.seg));
   };
 
+  // Vectors of a segment of n that pass B finds no more in the ring.
+  auto lost = [&](int n) { return max(0, (n + job.sub - 1) / job.sub - job.stages) * job.sub; };
+
   // The copies run ahead of the work by what the ring holds: `ahead` is the
   // live item they are at, `done` of its `count` vectors are loaded or on their
-  // way.
-  int ahead = group, done = 0, count = 0;
+  // way, and the first `again` are to be loaded a second time.
+  int ahead = group, done = 0, count = 0, again = 0;
   const uint4* src = nullptr;
   auto open_ahead = [&] {
     if (ahead >= live) return;
     const int item = todo.live(ahead), part = part_of(item);
     done = 0;
     count = my_count(part);
+    if (kMode == kRowLong) again = lost(count);
     src = reinterpret_cast<const uint4*>(logits + row_of(item) * job.ld) + my_first(part);
   };
   open_ahead();
   auto load_next = [&] {
-    while (ahead < live && done >= count) ahead += groups, open_ahead();
+    while (ahead < live && done >= count) {
+      if (kMode == kRowLong && again > 0) done = 0, count = again, again = 0;
+      else ahead += groups, open_ahead();
+    }
     if (ahead >= live) return;
     ring.load(src + done, min(job.sub, count - done) * 16, lane);
     done += job.sub;
@@ -644,18 +657,20 @@ __global__ void __launch_bounds__(kRowThreads, 1) row_kernel(T* dlogits, const T
       xt = r.target >= 0 && r.target < job.V ? elem_to_float(logits[row * job.ld + r.target]) : NAN;
     }
     RunningSum run;
-    const int out0 = ring.out, loading0 = ring.loading;
-    const uint32_t phase0 = ring.out_phase;
+    const int gone = kMode == kRowGrad ? 0 : (kMode == kRowLong ? lost(n) : n);  // what lies before is given up as it is read
+    int out0 = ring.out, loading0 = ring.loading;
+    uint32_t phase0 = ring.out_phase;
     for (int c = 0; c < n; c += job.sub) {
+      if (kMode == kRowLong && c == gone) out0 = ring.out, phase0 = ring.out_phase, loading0 = ring.loading;
       ok = ok && ring.wait(4);
       const int nc = min(job.sub, n - c);
       if (!ok) break;
       const uint4* x = ring.chunk();
       const int full = min(nc, job.V / kV - v0 - c);
       if (c == 0) run.start(lane < full ? max_vec<T>(x[lane]) : -INFINITY);
-      run.add_all<T, kMode != kRowGrad || sizeof(T) == 4>(x, full, full < nc, job.V % kV, lane);
+      run.add_all<T, !kGrad || sizeof(T) == 4>(x, full, full < nc, job.V % kV, lane);
       ring.step();
-      if (kMode != kRowGrad) {
+      if (c < gone) {
         __syncwarp();
         load_next();
       }
@@ -672,22 +687,27 @@ __global__ void __launch_bounds__(kRowThreads, 1) row_kernel(T* dlogits, const T
       t.xt = xt;
       if (lane == 0) {
         job.slots[static_cast<long long>(part) * job.rows + row] = t;
-        if (kMode == kRowGrad) {
+        if (kGrad) {
           const float c = policy_coef(args, r, weight, t);
           coef[warp] = RowCoef{finite_max(t.m), c / static_cast<float>(t.s), c, r.target};
         }
       }
     }
     ++k;
-    if (kMode == kRowGrad) {
+    if (kGrad) {
       meet();
       const RowCoef rc = coef[group * G];
       T* d = dlogits + row * job.ld;
-      // back over the same chunks
-      ring.out = out0, ring.out_phase = phase0, ring.loading = loading0;
+      // back over the same chunks, then over those that come again
+      if (ok) ring.out = out0, ring.out_phase = phase0, ring.loading = loading0;
+      const int kept = kMode == kRowLong ? (n + job.sub - 1) / job.sub * job.sub - gone : n;
       if (ok && rc.c == 0.f) {
         zero_vecs(reinterpret_cast<uint4*>(d) + v0, n, lane, 32);
-        for (int c = 0; c < n; c += job.sub) {
+        for (int i = 0; i < n; i += job.sub) {
+          if (kMode == kRowLong) {
+            if (i >= kept) ok = ok && ring.wait(5);
+            if (!ok) break;
+          }
           ring.step();
           load_next();
         }
@@ -695,7 +715,12 @@ __global__ void __launch_bounds__(kRowThreads, 1) row_kernel(T* dlogits, const T
         const RowGradient<T> g(rc);
         float value = 0.f;  // the gradient at the target
         bool target_here = false;
-        for (int c = 0; c < n; c += job.sub) {
+        for (int i = 0; i < n; i += job.sub) {
+          const int c = kMode == kRowGrad ? i : (i < kept ? gone + i : i - kept);
+          if (kMode == kRowLong) {
+            if (i >= kept) ok = ok && ring.wait(5);
+            if (!ok) break;
+          }
           const int nc = min(job.sub, n - c);
           g.store(d, ring.chunk(), v0 + c, nc, job.V, lane);
           const int t = rc.target - (v0 + c) * kV;
@@ -713,7 +738,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) row_kernel(T* dlogits, const T
       zero_rows(static_cast<int>(static_cast<float>(at + 1) * per_live));
     }
   }
-  if (kMode == kRowGrad) zero_rows(n_items);
+  if (kGrad) zero_rows(n_items);
   ring.drain();
   if (kMode == kRowStats) return;
   // The losses of this CTA's rows, in 64 bits, a row a thread: beside the passes
@@ -950,10 +975,10 @@ int div_up(long long a, long long b) { return static_cast<int>((a + b - 1) / b);
 // part fit the 227 KB of an SM.
 constexpr int kWarpRingBytes = 9216;
 
-// Fills in group, seg, sub and stages for units of job.vecs vectors; false when
-// `keep` is asked (a unit stays in its group's rings) and it does not fit.
+// Fills in group, seg, sub and stages for units of job.vecs vectors; returns
+// whether a unit fits its group's rings, which it should with `keep`.
+constexpr int kWarpVecs = kWarpRingBytes / 16;
 bool share_out(RowJob* job, bool keep) {
-  const int warp_vecs = kWarpRingBytes / 16;
   const long long units = static_cast<long long>(job->rows) * job->parts;
   static const int kGroups[] = {1, 2, 3, 4, 6, 8, 12, 24};  // the divisors of kRowWarps
   // the fewest warps a unit fits (or fits twice, when it only streams through:
@@ -961,16 +986,15 @@ bool share_out(RowJob* job, bool keep) {
   // work on rows of their own and one's barriers are hidden by the others (a warp
   // for itself, on parts of rows: 84 us, and 8192 rows of fp32 297 against 253 us), ...
   int g = 0;
-  while (kGroups[g] < kRowWarps && job->vecs > kGroups[g] * warp_vecs * (keep ? 1 : 2)) ++g;
-  if (keep && job->vecs > kGroups[g] * warp_vecs) return false;
+  while (kGroups[g] < kRowWarps && job->vecs > kGroups[g] * kWarpVecs * (keep ? 1 : 2)) ++g;
   // ... and more when there are so few units that every one still has its group
   while (kGroups[g] < kRowWarps && units * kGroups[g + 1] <= static_cast<long long>(num_sms()) * kRowWarps && job->vecs > 32 * kGroups[g]) ++g;
   job->group = kGroups[g];
   job->seg = div_up(job->vecs, job->group);
   const int chunks = std::max(1, std::min(div_up(job->seg, 192), 3));
   job->sub = std::min(div_up(div_up(job->seg, chunks), 32) * 32, 192);
-  job->stages = std::min(kMaxStages, warp_vecs / job->sub);
-  return !keep || job->stages * job->sub >= job->seg;
+  job->stages = std::min(kMaxStages, kWarpVecs / job->sub);
+  return job->stages * job->sub >= job->seg;
 }
 
 template <typename T, int kMode>
@@ -1037,7 +1061,14 @@ int policy_loss(void* dlogits, const void* logits, const PolicyArgs& a, int rows
     share_out(&job, false);
     return launch_rows<T, kRowEval>(nullptr, logits, job, a, s);
   }
-  if (share_out(&job, true)) return launch_rows<T, kRowGrad>(dlogits, logits, job, a, s);
+  // Rows that take more than half an SM each, and for at most half the SMs: three
+  // kernels over parts of rows on all SMs are faster (16 rows of 131072 bf16: 11.3
+  // against 19.4 us, 64: 16.0 against 19.9, 96: 21.2 against 21.1; 64 of 100000:
+  // 14.5 against 16.0, 96: 17.4 against 16.5; 64 of 50257: the same).
+  if (job.vecs <= kRowWarps / 2 * kWarpVecs || 2 * rows > num_sms()) {
+    const bool fits = share_out(&job, true);
+    return fits ? launch_rows<T, kRowGrad>(dlogits, logits, job, a, s) : launch_rows<T, kRowLong>(dlogits, logits, job, a, s);
+  }
   RowSum* slots = job.slots;
   auto* coefs = reinterpret_cast<RowCoef*>(static_cast<char*>(workspace) + slots_bytes(rows, Vp));
   int nslots = 0;

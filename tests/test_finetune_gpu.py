@@ -133,6 +133,28 @@ def test_policy_loss(cuda_dev, shape, dt):
     p.check()
 
 
+@pytest.mark.parametrize("rows,V,Vp,dt", [(90, 131072, 131080, torch.bfloat16), (301, 110593, 110600, torch.bfloat16),
+                                          (80, 400001, 400008, torch.bfloat16), (160, 55297, 55304, torch.float32),
+                                          (75, 200003, 200008, torch.float32), (74, 131072, 131072, torch.bfloat16)])
+def test_policy_loss_long_rows(cuda_dev, rows, V, Vp, dt):
+    """Rows that do not fit an SM's shared memory, by one kernel and (few of them) by three."""
+    p = Policy(rows, V, Vp, dt, cuda_dev, seed=rows)
+    n = V // 7
+    for i in range(0, rows, 3):  # targets in every stretch of a row, its ends included
+        p.t[i] = min(V - 1, (i // 3) % 8 * n) if i % 2 else V - 1 - min(V - 1, (i // 3) % 8 * n)
+    _, lp = logps_of(p.x, p.t, V)
+    p.old, p.ref = (lp + 0.05).float(), (lp - 0.1).float()
+    p.call()
+    p.check()
+    p.kl, p.A[1::2] = 0.0, 0.0  # every other live row without a gradient
+    p.call()
+    p.check()
+    assert (p.dx[1::2] == 0).all()
+    y = p.x.clone()
+    p.call(logits=y, dlogits=y)
+    assert torch.equal(y, p.dx)
+
+
 @pytest.mark.parametrize("kw", [dict(old=False), dict(ref=False, kl=0.0), dict(kl=0.0), dict(masked=0.0),
                                 dict(lo=0.0, hi=0.0), dict(lo=1.0, hi=5.0), dict(old=False, ref=False, kl=0.0)])
 def test_policy_loss_forms(cuda_dev, kw):
