@@ -747,12 +747,10 @@ __global__ void __launch_bounds__(kRowThreads, 1) row_kernel(T* dlogits, const T
   for (int i = threadIdx.x; i < n_items; i += kRowThreads) {
     const long long row = row_of(i);
     const float weight = job.weights ? job.weights[row] : 1.f;
-    if (weight == 0.f) {
-      policy_row_masked(args, row);
-    } else {
-      const RowSum t = job.slots[row];
-      policy_row(args, policy_row_load(args, row), row, weight, logp_of(t));
-    }
+    const RowSum t = job.slots[row];  // all loads at once, for nothing in masked rows
+    const PolicyRow r = policy_row_load(args, row);
+    if (weight == 0.f) policy_row_masked(args, row);
+    else policy_row(args, r, row, weight, logp_of(t));
   }
 }
 
@@ -976,23 +974,37 @@ int div_up(long long a, long long b) { return static_cast<int>((a + b - 1) / b);
 constexpr int kWarpRingBytes = 9216;
 
 // Fills in group, seg, sub and stages for units of job.vecs vectors; returns
-// whether a unit fits its group's rings, which it should with `keep`.
+// whether a unit fits its group's rings.
+//
+// Of the groups whose rings hold a unit `times` over, the one that is through
+// first, in rounds of units on all SMs: a unit costs its warps their share of the
+// vectors and as much again as 300 vectors for the joining of their sums (from
+// times of 320 to 16384 rows). times: 1 where a unit stays in the rings. Where it
+// streams through them, larger units in smaller groups leave more groups to work
+// while one joins, down to a fifth in bf16, where instructions count as much as
+// HBM (8192 rows of 50257 133 us, by groups of half a unit 145; 4096 of 131072
+// 178 against 222), and a half in fp32, where HBM does (1500 pair rows 242 us, 258
+// by smaller groups). Chunks are as large as a ring of two allows: each costs a
+// wait, a copy and a start of the loops (192 vectors instead of 288: 8192 rows of
+// 20000 149 against 136 us, evaluation of 50257 149 against 141; 96: 166 us).
 constexpr int kWarpVecs = kWarpRingBytes / 16;
-bool share_out(RowJob* job, bool keep) {
+template <typename T>
+constexpr int kStream = sizeof(T) == 2 ? 5 : 2;
+bool share_out(RowJob* job, int times) {
   const long long units = static_cast<long long>(job->rows) * job->parts;
   static const int kGroups[] = {1, 2, 3, 4, 6, 8, 12, 24};  // the divisors of kRowWarps
-  // the fewest warps a unit fits (or fits twice, when it only streams through:
-  // evaluation of 4096 rows 79 us, 87 us by groups it fits once), so that groups
-  // work on rows of their own and one's barriers are hidden by the others (a warp
-  // for itself, on parts of rows: 84 us, and 8192 rows of fp32 297 against 253 us), ...
-  int g = 0;
-  while (kGroups[g] < kRowWarps && job->vecs > kGroups[g] * kWarpVecs * (keep ? 1 : 2)) ++g;
-  // ... and more when there are so few units that every one still has its group
-  while (kGroups[g] < kRowWarps && units * kGroups[g + 1] <= static_cast<long long>(num_sms()) * kRowWarps && job->vecs > 32 * kGroups[g]) ++g;
-  job->group = kGroups[g];
+  long long best = 0;
+  job->group = 0;
+  for (int group : kGroups) {
+    if (group < kRowWarps && job->vecs > group * times * kWarpVecs) continue;
+    if (job->group && job->vecs <= 32 * job->group) break;
+    const long long at_once = static_cast<long long>(num_sms()) * (kRowWarps / group);
+    const long long cost = (units + at_once - 1) / at_once * (div_up(job->vecs, group) + 300);
+    if (!job->group || cost < best) job->group = group, best = cost;
+  }
   job->seg = div_up(job->vecs, job->group);
-  const int chunks = std::max(1, std::min(div_up(job->seg, 192), 3));
-  job->sub = std::min(div_up(div_up(job->seg, chunks), 32) * 32, 192);
+  const int chunks = std::min(div_up(job->seg, kWarpVecs / 2), 2);
+  job->sub = std::min(div_up(div_up(job->seg, chunks), 32) * 32, kWarpVecs / 2);
   job->stages = std::min(kMaxStages, kWarpVecs / job->sub);
   return job->stages * job->sub >= job->seg;
 }
@@ -1034,7 +1046,7 @@ int launch_slots(RowSum* slots, int* nslots, const void* logits, const float* we
   job.slots = slots;
   job.vecs = div_up(all, parts_of(rows, V));
   job.parts = *nslots = div_up(all, job.vecs);  // rounding up may leave the last part empty
-  share_out(&job, false);
+  share_out(&job, kStream<T>);
   return launch_rows<T, kRowStats>(nullptr, logits, job, PolicyArgs{}, s);
 }
 
@@ -1058,7 +1070,7 @@ int policy_loss(void* dlogits, const void* logits, const PolicyArgs& a, int rows
   RowJob job = row_job<T>(a.weights, rows, V, Vp);
   job.slots = static_cast<RowSum*>(workspace);
   if (!dlogits) {
-    share_out(&job, false);
+    share_out(&job, kStream<T>);
     return launch_rows<T, kRowEval>(nullptr, logits, job, a, s);
   }
   // Rows that take more than half an SM each, and for at most half the SMs: three
@@ -1066,7 +1078,7 @@ int policy_loss(void* dlogits, const void* logits, const PolicyArgs& a, int rows
   // against 19.4 us, 64: 16.0 against 19.9, 96: 21.2 against 21.1; 64 of 100000:
   // 14.5 against 16.0, 96: 17.4 against 16.5; 64 of 50257: the same).
   if (job.vecs <= kRowWarps / 2 * kWarpVecs || 2 * rows > num_sms()) {
-    const bool fits = share_out(&job, true);
+    const bool fits = share_out(&job, 1);
     return fits ? launch_rows<T, kRowGrad>(dlogits, logits, job, a, s) : launch_rows<T, kRowLong>(dlogits, logits, job, a, s);
   }
   RowSum* slots = job.slots;
