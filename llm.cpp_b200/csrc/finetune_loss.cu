@@ -323,6 +323,29 @@ struct RunningSum {
   }
 };
 
+// The same over a warp's only chunk by expf, added in 64 bits, with nothing to
+// correct: `off` is what `s` rounds away, `part` 0.
+template <typename T>
+__device__ __forceinline__ WarpSum exact_sum(const uint4* x, int full, bool partial, int keep, int lane) {
+  float top = -INFINITY;
+  for (int i = lane; i < full; i += 32) top = fmaxf(top, max_vec<T>(x[i]));
+  if (partial && lane == 0) top = fmaxf(top, max_vec<T>(cut_vec<T>(x[full], keep)));
+  top = warp_max_f(top);
+  const float ref = finite_max(top);
+  double s = 0.0;
+  auto add = [&](const uint4& u) {
+    float v[vec_elems<T>()];
+    unpack_vec(u, v);
+#pragma unroll
+    for (int j = 0; j < vec_elems<T>(); ++j) s += static_cast<double>(expf(v[j] - ref));
+  };
+  for (int i = lane; i < full; i += 32) add(x[i]);
+  if (partial && lane == 0) add(cut_vec<T>(x[full], keep));
+  s = warp_sum_d(s);
+  const float high = static_cast<float>(s);
+  return WarpSum{top, top, high, 0.f, static_cast<float>(s - static_cast<double>(high))};
+}
+
 // A row's sum from sums over its warps, at its maximum M. `off / part` is what
 // the terms lack; expf itself is 6e-9 high on average, in the terms computed
 // twice and in the warps' factors. The maximum's own term is exactly 1 and needs
@@ -335,6 +358,13 @@ __device__ __forceinline__ RowSum corrected(float M, float sum, float part, floa
 }
 // A row's sum from one warp's, or from several (lanes >= count: none); the same
 // in every lane.
+__device__ __forceinline__ RowSum fold_exact(const WarpSum* sums, int count, int lane) {
+  WarpSum w{-INFINITY, -INFINITY, 0.f, 0.f, 0.f};
+  if (lane < count) w = sums[lane];
+  const float M = warp_max_f(w.top);
+  const double f = exp(static_cast<double>(w.top) - static_cast<double>(finite_max(M)));
+  return RowSum{warp_sum_d((static_cast<double>(w.s) + static_cast<double>(w.off)) * f), M, 0.f};
+}
 __device__ __forceinline__ RowSum fold_warp(const WarpSum& w) {
   const float f = expf(w.m - finite_max(w.top));
   return corrected(w.top, w.s * f, w.part, w.off);
@@ -533,7 +563,8 @@ struct RowList {
 enum RowMode { kRowGrad, kRowLong, kRowEval, kRowStats };
 
 // How row_kernel shares the work out. A unit is a row, or (kRowStats) one of
-// `parts` parts of it, of `vecs` vectors; a launch covers units [unit0, unit1) of
+// `parts` parts of it, of `vecs` vectors, summed by expf (`exact`) or by
+// ex2.approx; a launch covers units [unit0, unit1) of
 // rows * parts, CTA b those at unit0 + b, unit0 + b + grid, ...; `group` warps
 // take a unit, each `seg` vectors of it, through its ring in chunks of `sub`.
 struct RowJob {
@@ -542,6 +573,7 @@ struct RowJob {
   int rows, V, ld;
   unsigned unit0, unit1;
   int parts, vecs, group, seg, sub, stages;
+  bool exact;
   unsigned int* status;
 };
 
@@ -559,7 +591,7 @@ struct RowJob {
 // Masked rows take no chunk. Each unit's (max, sum) goes to its
 // slot, planes of `rows`. A wait that is given up (the device status says so)
 // ends the work, not the barriers: the group's warps still meet.
-template <typename T, int kMode>
+template <typename T, int kMode, bool kExact>
 __global__ void __launch_bounds__(kRowThreads, 1) row_kernel(T* dlogits, const T* logits, RowJob job, PolicyArgs args) {
   constexpr int kV = vec_elems<T>();
   constexpr bool kGrad = kMode == kRowGrad || kMode == kRowLong;
@@ -657,6 +689,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) row_kernel(T* dlogits, const T
       xt = r.target >= 0 && r.target < job.V ? elem_to_float(logits[row * job.ld + r.target]) : NAN;
     }
     RunningSum run;
+    WarpSum sum{-INFINITY, -INFINITY, 0.f, 0.f, 0.f};
     const int gone = kMode == kRowGrad ? 0 : (kMode == kRowLong ? lost(n) : n);  // what lies before is given up as it is read
     int out0 = ring.out, loading0 = ring.loading;
     uint32_t phase0 = ring.out_phase;
@@ -667,23 +700,28 @@ __global__ void __launch_bounds__(kRowThreads, 1) row_kernel(T* dlogits, const T
       if (!ok) break;
       const uint4* x = ring.chunk();
       const int full = min(nc, job.V / kV - v0 - c);
-      if (c == 0) run.start(lane < full ? max_vec<T>(x[lane]) : -INFINITY);
-      run.add_all<T, !kGrad || sizeof(T) == 4>(x, full, full < nc, job.V % kV, lane);
+      if constexpr (kExact) {
+        sum = exact_sum<T>(x, full, full < nc, job.V % kV, lane);
+      } else {
+        if (c == 0) run.start(lane < full ? max_vec<T>(x[lane]) : -INFINITY);
+        run.add_all<T, !kGrad || sizeof(T) == 4>(x, full, full < nc, job.V % kV, lane);
+      }
       ring.step();
       if (c < gone) {
         __syncwarp();
         load_next();
       }
     }
-    const WarpSum sum = run.join();
+    if constexpr (!kExact) sum = run.join();
     // Two sets of sums: a set is rewritten two rows on, and between lies a
     // meeting that the group's first warp reaches only after reading it.
-    if (G > 1) {
+    if (G > 1 || kExact) {
       if (lane == 0) sums[k & 1][warp] = sum;
       meet();
     }
     if (gw == 0) {
-      RowSum t = G > 1 ? fold_warps(&sums[k & 1][warp], G, lane) : fold_warp(sum);
+      RowSum t = kExact ? fold_exact(&sums[k & 1][warp], G, lane)
+                           : (G > 1 ? fold_warps(&sums[k & 1][warp], G, lane) : fold_warp(sum));
       t.xt = xt;
       if (lane == 0) {
         job.slots[static_cast<long long>(part) * job.rows + row] = t;
@@ -1006,20 +1044,28 @@ bool share_out(RowJob* job, int times) {
   const int chunks = std::min(div_up(job->seg, kWarpVecs / 2), 2);
   job->sub = std::min(div_up(div_up(job->seg, chunks), 32) * 32, kWarpVecs / 2);
   job->stages = std::min(kMaxStages, kWarpVecs / job->sub);
+  // One round of a few vectors: sums by expf and in 64 bits cost 0.1 to 0.9 us there
+  // (148 rows of 500 to 20000; 73 us of 132 in 8192 rows of 50257), and single rows
+  // of few terms, whose rounding errors do not average out, need them: KL estimates
+  // of one row of 1572 were 2e-6 off, and are 2e-7.
+  job->exact = job->seg <= 128 && units <= static_cast<long long>(num_sms()) * (kRowWarps / job->group);
   return job->stages * job->sub >= job->seg;
 }
 
-template <typename T, int kMode>
+template <typename T, int kMode, bool kExact = false>
 int launch_rows(void* dlogits, const void* logits, const RowJob& job, const PolicyArgs& a, cudaStream_t s) {
+  if constexpr (!kExact && kMode != kRowLong) {
+    if (job.exact) return launch_rows<T, kMode, true>(dlogits, logits, job, a, s);
+  }
   static bool done[64] = {};
-  LLMK_TRY(allow_smem(row_kernel<T, kMode>, kRowWarps * kWarpRingBytes, done));
+  LLMK_TRY(allow_smem(row_kernel<T, kMode, kExact>, kRowWarps * kWarpRingBytes, done));
   const size_t smem = static_cast<size_t>(kRowWarps) * job.stages * job.sub * 16;
   const long long units = static_cast<long long>(job.rows) * job.parts, most = static_cast<long long>(num_sms()) * kMaxItems;
   for (long long u = 0; u < units; u += most) {
     RowJob now = job;
     now.unit0 = static_cast<unsigned>(u);
     now.unit1 = static_cast<unsigned>(std::min(units, u + most));
-    row_kernel<T, kMode><<<static_cast<int>(std::min<long long>(now.unit1 - now.unit0, num_sms())), kRowThreads, smem, s>>>(
+    row_kernel<T, kMode, kExact><<<static_cast<int>(std::min<long long>(now.unit1 - now.unit0, num_sms())), kRowThreads, smem, s>>>(
         static_cast<T*>(dlogits), static_cast<const T*>(logits), now, a);
     count_launch();
   }

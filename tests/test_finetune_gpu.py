@@ -133,6 +133,21 @@ def test_policy_loss(cuda_dev, shape, dt):
     p.check()
 
 
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,V,Vp", [(1, 7, 8), (2, 1555, 1696), (3, 501, 504), (8, 2000, 2000), (100, 5000, 5000)])
+def test_few_rows_of_small_vocabularies(cuda_dev, rows, V, Vp, dt, monkeypatch):
+    """Here a log-probability is off by at most 40 u: expf 2 u, the difference it is of 8 u (in the mean over the terms,
+    8 apart), 8 additions in a lane, 5 in a warp and 5 over warps, and two factors expf(m - max) of 3 u; in all 34 u."""
+    import sys
+    monkeypatch.setattr(sys.modules[__name__], "LP", 40 * U)
+    for grad in (True, False):
+        p = Policy(rows, V, Vp, dt, cuda_dev, seed=V + rows, masked=0.0)
+        if not grad:
+            p.dx = None
+        p.call()
+        p.check()
+
+
 @pytest.mark.parametrize("rows,V,Vp,dt", [(90, 131072, 131080, torch.bfloat16), (301, 110593, 110600, torch.bfloat16),
                                           (80, 400001, 400008, torch.bfloat16), (160, 55297, 55304, torch.float32),
                                           (75, 200003, 200008, torch.float32), (74, 131072, 131072, torch.bfloat16)])
