@@ -843,10 +843,12 @@ __global__ void __launch_bounds__(kPairThreads) preference_pair_kernel(RowCoef* 
   };
   if (kEarly) fetch(first);
   grid_wait();
-  // before the barrier that the outputs come after: rewards may be ref_logps
+  // before the barrier that the outputs come after: rewards may be ref_logps, and
+  // so may logps where a sequence is one row (elsewhere their sizes differ)
   const float ref0 = a.ref_logps ? a.ref_logps[pair] : 0.f, ref1 = a.ref_logps ? a.ref_logps[pairs + pair] : 0.f;
   double sum = 0.0;
   RowCoef mine{0.f, 0.f, 0.f, -1};  // of the thread's first row; the others' wait in memory
+  float logp = 0.f;                 // as well
   for (int t = first; t < Tlen; t += kSide) {
     const long long row = row0 + t;
     if (!kEarly || t != first) fetch(t);
@@ -854,13 +856,18 @@ __global__ void __launch_bounds__(kPairThreads) preference_pair_kernel(RowCoef* 
     const double lp = w != 0.f ? logp_of(f) : 0.0;
     if (w != 0.f) sum += static_cast<double>(w) * lp;
     const RowCoef c{finite_max(f.m), static_cast<float>(1.0 / f.s), w, target};
-    if (t == first) mine = c;
-    else if (coefs) coefs[row] = c;
-    if (a.logps) a.logps[row] = static_cast<float>(lp);
+    if (t == first) {
+      mine = c;
+      logp = static_cast<float>(lp);
+    } else {
+      if (coefs) coefs[row] = c;
+      if (a.logps) a.logps[row] = static_cast<float>(lp);
+    }
   }
   sum = warp_sum_d(sum);
   if (lane == 0) red[side][first / 32] = sum;
   __syncthreads();
+  if (a.logps && first < Tlen) a.logps[row0 + first] = logp;
   const double L0 = warp_sum_d(lane < kSide / 32 ? red[0][lane] : 0.0), L1 = warp_sum_d(lane < kSide / 32 ? red[1][lane] : 0.0);
   const double beta = a.beta, eps = a.smoothing;
   const double rc = beta * (L0 - static_cast<double>(ref0)), rr = beta * (L1 - static_cast<double>(ref1));
