@@ -95,12 +95,11 @@ __device__ __forceinline__ double logp_of(const RowSum& t) {
   return static_cast<double>(t.xt) - static_cast<double>(t.m) - log(t.s);
 }
 
-// The policy loss of one live row, given lp: writes the row's outputs and
-// returns d(loss)/d(lp) with weight and dscale. With rho = exp(lp - old), A the
-// advantage and d = ref - lp: loss = w (-min(rho A, clamp(rho) A) + kl_coef
-// (exp(d) - d - 1)). The clipped branch has no gradient; where both products are
-// equal (rho inside the bounds, or on one) the unclipped one counts. In 64 bits:
-// exp(d) - d - 1 is a difference of nearly equal numbers for a policy close to
+// The policy loss of one live row. With rho = exp(lp - old), A the advantage and
+// d = ref - lp: loss = w (-min(rho A, clamp(rho) A) + kl_coef (exp(d) - d - 1)).
+// The clipped branch has no gradient; where both products are equal (rho inside
+// the bounds, or on one) the unclipped one counts. In 64 bits: exp(d) - 1 and
+// exp(d) - d - 1 are differences of nearly equal numbers for a policy close to
 // its reference, and rho against a bound decides between two gradients.
 struct PolicyRow {
   float adv, old, ref;
@@ -114,14 +113,27 @@ __device__ __forceinline__ PolicyRow policy_row_load(const PolicyArgs& a, long l
   r.target = a.targets[row];
   return r;
 }
-__device__ __forceinline__ double policy_row(const PolicyArgs& a, const PolicyRow& r, long long row, float w, double lp) {
-  const double A = r.adv;
-  const double rho = a.old_logps ? exp(lp - static_cast<double>(r.old)) : 1.0;
+// -min(rho A, clamp(rho) A) and its derivative by lp. The loss and the gradient
+// take rho = exp(xt - max - old) / sum from the same operations, so that they
+// decide alike.
+struct PolicyTerm {
+  double loss, slope;
+};
+__device__ __forceinline__ PolicyTerm policy_term(const PolicyArgs& a, double A, double rho) {
   const double lo = 1.0 - static_cast<double>(a.clip_low), hi = 1.0 + static_cast<double>(a.clip_high);
   const double clamped = rho < lo ? lo : (rho > hi ? hi : rho);
   const double s1 = A == 0.0 ? 0.0 : rho * A, s2 = clamped * A;
-  double loss = s1 > s2 ? -s2 : -s1;
-  double g = s1 > s2 ? 0.0 : -s1;
+  return s1 > s2 ? PolicyTerm{-s2, 0.0} : PolicyTerm{-s1, -s1};
+}
+__device__ __forceinline__ double target_offset(const RowSum& t) {  // lp + log(sum)
+  return static_cast<double>(t.xt) - static_cast<double>(t.m);
+}
+// Writes the row's outputs and returns d(loss)/d(lp) with weight and dscale.
+__device__ __forceinline__ double policy_row(const PolicyArgs& a, const PolicyRow& r, long long row, float w, const RowSum& t) {
+  const double lp = logp_of(t);
+  const double rho = a.old_logps ? exp(target_offset(t) - static_cast<double>(r.old)) * (1.0 / t.s) : 1.0;
+  const PolicyTerm term = policy_term(a, r.adv, rho);
+  double loss = term.loss, g = term.slope;
   if (isnan(lp)) loss = g = lp;  // also where rho does not carry it
   if (a.ref_logps) {
     const double d = static_cast<double>(r.ref) - lp;
@@ -137,28 +149,20 @@ __device__ __forceinline__ double policy_row(const PolicyArgs& a, const PolicyRo
   if (a.logps) a.logps[row] = static_cast<float>(lp);
   return g * w * a.dscale;
 }
-// The same coefficient in fp32, for the gradient: rho = exp(xt - max - old) / sum
-// and exp(d) = exp(ref - xt + max) sum need no logarithm, and two exponentials
-// side by side take a fourth of policy_row's time, which the row's warps would
-// wait for. Off by a few steps of fp32, as the exponentials it multiplies.
-__device__ __forceinline__ float policy_coef(const PolicyArgs& a, const PolicyRow& r, float w, const RowSum& t) {
-  auto exp_d = [](double v) {  // exp of a difference that one float does not hold
-    const float h = static_cast<float>(v);
-    return expf(h) * (1.f + (isfinite(h) ? static_cast<float>(v - static_cast<double>(h)) : 0.f));
-  };
-  const double x = static_cast<double>(t.xt) - static_cast<double>(t.m);
-  const float s = static_cast<float>(t.s);
-  const bool lost = isnan(x) || isnan(s);
-  float rho = 1.f;
-  if (a.old_logps) {
-    const double v = x - static_cast<double>(r.old);
-    rho = v > 80.0 ? exp_d(v - 64.0) * (6.2351491e27f / s) : exp_d(v) / s;  // e^64: a ratio that fp32 holds
+// The coefficient alone, by a whole warp, while the row's other warps wait: no
+// logarithm, since exp(d) = exp(ref - xt + max) sum, and one exponential for both
+// terms, of lane 0 for rho and of the others for the KL term.
+__device__ __forceinline__ double policy_coef(const PolicyArgs& a, const PolicyRow& r, float w, const RowSum& t, double inv_s, int lane) {
+  const double x = target_offset(t);
+  double rho = 1.0, e = 0.0;
+  if (a.old_logps || a.kl_coef != 0.f) {
+    const double v = exp(lane == 0 ? x - static_cast<double>(r.old) : static_cast<double>(r.ref) - x);
+    if (a.old_logps) rho = __shfl_sync(0xffffffffu, v, 0) * inv_s;
+    e = __shfl_sync(0xffffffffu, v, 1) * t.s - 1.0;
   }
-  const float clamped = fminf(fmaxf(rho, 1.f - a.clip_low), 1.f + a.clip_high);
-  const float s1 = r.adv == 0.f ? 0.f : rho * r.adv, s2 = clamped * r.adv;
-  float g = s1 > s2 ? 0.f : -s1;
-  if (a.kl_coef != 0.f) g -= a.kl_coef * (exp_d(static_cast<double>(r.ref) - x) * s - 1.f);
-  return lost ? NAN : g * w * a.dscale;
+  double g = policy_term(a, r.adv, rho).slope;
+  if (a.kl_coef != 0.f) g -= static_cast<double>(a.kl_coef) * e;
+  return isnan(x) || isnan(t.s) ? static_cast<double>(NAN) : g * w * a.dscale;
 }
 __device__ __forceinline__ void policy_row_masked(const PolicyArgs& a, long long row) {
   a.losses[row] = 0.f;
@@ -723,12 +727,10 @@ __global__ void __launch_bounds__(kRowThreads, 1) row_kernel(T* dlogits, const T
       RowSum t = kExact ? fold_exact(&sums[k & 1][warp], G, lane)
                            : (G > 1 ? fold_warps(&sums[k & 1][warp], G, lane) : fold_warp(sum));
       t.xt = xt;
-      if (lane == 0) {
-        job.slots[static_cast<long long>(part) * job.rows + row] = t;
-        if (kGrad) {
-          const float c = policy_coef(args, r, weight, t);
-          coef[warp] = RowCoef{finite_max(t.m), c / static_cast<float>(t.s), c, r.target};
-        }
+      if (lane == 0) job.slots[static_cast<long long>(part) * job.rows + row] = t;
+      if (kGrad) {
+        const double inv_s = 1.0 / t.s, c = policy_coef(args, r, weight, t, inv_s, lane);
+        if (lane == 0) coef[warp] = RowCoef{finite_max(t.m), static_cast<float>(c * inv_s), static_cast<float>(c), r.target};
       }
     }
     ++k;
@@ -788,7 +790,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) row_kernel(T* dlogits, const T
     const RowSum t = job.slots[row];  // all loads at once, for nothing in masked rows
     const PolicyRow r = policy_row_load(args, row);
     if (weight == 0.f) policy_row_masked(args, row);
-    else policy_row(args, r, row, weight, logp_of(t));
+    else policy_row(args, r, row, weight, t);
   }
 }
 
@@ -810,7 +812,7 @@ __global__ void __launch_bounds__(128) policy_rows_kernel(RowCoef* __restrict__ 
     if (coefs) coefs[row] = RowCoef{0.f, 0.f, 0.f, -1};
     return;
   }
-  const double c = policy_row(a, r, row, w, logp_of(t));
+  const double c = policy_row(a, r, row, w, t);
   if (coefs) coefs[row] = RowCoef{finite_max(t.m), static_cast<float>(c / t.s), static_cast<float>(c), r.target};
 }
 

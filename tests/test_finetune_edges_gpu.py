@@ -1,9 +1,12 @@
 """Calls of the fine-tuning operators at the edges of what their documentation
 allows, on the GPU."""
+import math
+
+import numpy as np
 import pytest
 import torch
 
-from test_finetune_gpu import Preference
+from test_finetune_gpu import Policy, Preference
 
 pytestmark = pytest.mark.gpu
 
@@ -26,3 +29,67 @@ def test_log_probabilities_over_the_reference_of_one_row_sequences(cuda_dev, pai
         q.ref.copy_(ref)
         q.call(logps=q.ref, weights=w, rewards=w)
         assert all(torch.equal(a, b) for a, b in zip(want, (q.losses, w, q.ref, q.dx)))
+
+
+U = 2.0 ** -24
+LEAN = 1.2e-8  # what the sum of a long row may be off by in the mean (its correction by expf's own), relative
+ROWS = [(5, 1001, 1008), (300, 1001, 1008), (5000, 40, 40), (40, 50257, 50304), (200, 50257, 50304), (90, 131072, 131080),
+        (3, 131072, 131080)]
+
+
+def two_tokens(shape, dt, dev, **kw):
+    """Rows whose whole mass lies on the target and on one other token, in equal parts: lp = -log 2 exactly, and the
+    gradient is c / 2 at the one and -c / 2 at the other."""
+    rows, V, Vp = shape
+    p = Policy(rows, V, Vp, dt, dev, seed=rows + V, masked=0.0, **kw)
+    p.x[:, :V] = -math.inf
+    at = torch.arange(rows, device=dev)
+    p.t[:] = (at * 37 % V).int()
+    other = (at * 37 + 1 + at % (V - 1)) % V
+    p.x[at, p.t.long()], p.x[at, other] = 0.0, 0.0
+    return p, at, other
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", ROWS)
+def test_policy_gradient_next_to_the_reference(cuda_dev, shape, dt):
+    """Where the KL term is the whole gradient (advantage 0, or a clipped ratio) and the policy is next to its reference,
+    that gradient is 1 - exp(d): no error of exp(d) itself may reach it. c is off by what the row's sum is (LEAN for
+    d), and the results by three roundings of c or c / sum, against half of c, and by one to their type; 16-bit ones also by a
+    step of log2 (c / sum), 32 u at 16 to 32, in the exponent, and by 4 u of the exponential."""
+    p, at, other = two_tokens(shape, dt, cuda_dev, kl=0.5)
+    rows = shape[0]
+    size = torch.tensor([1e-5, -1e-5, 1e-4, -1e-4, 1e-3, -1e-3], device=cuda_dev, dtype=torch.float64)[at % 6]
+    p.ref = (size * (1 + torch.rand(rows, device=cuda_dev, dtype=torch.float64)) - math.log(2)).float()
+    # no policy term: advantage 0; a ratio of e^0.5 for a positive advantage, of e^-0.5 for a negative one
+    p.A = torch.tensor([0.0, 1.0, -1.0], device=cuda_dev)[(at // 6) % 3]
+    p.old = (-math.log(2) - 0.5 * p.A.double()).float()
+    p.call()
+    d = p.ref.double() + math.log(2)
+    k = p.w.double() * p.kl * float(np.float32(p.dscale))
+    want = -k * torch.expm1(d) / 2
+    tol = want.abs() * ((8 if dt == torch.float32 else 40) * U + torch.finfo(dt).eps / 2) + k * LEAN
+    for got, sign in ((p.dx[at, p.t.long()], 1), (p.dx[at, other], -1)):
+        assert ((sign * got.double() - want).abs() <= tol).all()
+    p.dx[at, p.t.long()], p.dx[at, other] = 0.0, 0.0
+    assert (p.dx == 0).all()
+
+
+@pytest.mark.parametrize("shape", ROWS)
+def test_policy_loss_and_gradient_take_the_same_branch(cuda_dev, shape):
+    """Ratios within a few steps of fp32 of a clipping bound: whether the gradient vanishes and whether the loss is the
+    clipped one go by the ratio in 64 bits."""
+    p, at, other = two_tokens(shape, torch.float32, cuda_dev, ref=False, kl=0.0)
+    lo, hi = 1 - float(np.float32(p.lo)), 1 + float(np.float32(p.hi))
+    p.A = torch.where(at % 2 == 0, 1.0, -1.0)
+    limit = torch.tensor([hi, lo], dtype=torch.float64, device=cuda_dev)[at % 2]
+    bound = -math.log(2) - torch.log(limit)
+    p.old = bound.float() + (at // 2 % 17 - 8) * 2.0 ** -24  # a step of fp32 at 0.5 to 1
+    past = torch.where(at % 2 == 0, 1.0, -1.0).double() * (bound - p.old.double())  # > 0: outside
+    near = past.abs() < 2 * LEAN  # what the row's sum may decide
+    p.call()
+    rho = torch.exp(-math.log(2) - p.old.double())
+    zero = (p.dx[at, p.t.long()] == 0) & (p.dx[at, other] == 0)
+    assert torch.equal(zero[~near], (past > 0)[~near])
+    loss = -p.w.double() * p.A.double() * torch.where(past > 0, limit, rho)
+    assert ((p.losses.double() - loss).abs() <= loss.abs() * (U + 2 * LEAN)).all()
