@@ -363,18 +363,28 @@ void with_table(const llmk_tensor* tensors, const Span& s, F f) {
   }
 }
 
-// Squares of every tensor; returns the number of partials.
-int launch_squares(double* partial, const llmk_tensor* tensors, const std::vector<Span>& spans, cudaStream_t s) {
+template <int kCap>
+cudaError_t launch_squares_of(int grid, cudaStream_t s, double* partial, const TensorTable<kCap>& tab) {
+  void* args[] = {&partial, const_cast<TensorTable<kCap>*>(&tab)};
+  return cudaLaunchKernel(reinterpret_cast<const void*>(&grad_squares_kernel<kCap>), dim3(grid), dim3(kThreads), args, 0, s);
+}
+
+// Squares of every tensor, their number of partials to *partials. A launch that
+// is refused ends the call: what follows would scale by what the workspace held.
+int launch_squares(int* partials, double* partial, const llmk_tensor* tensors, const std::vector<Span>& spans, cudaStream_t s) {
   int n = 0;
   for (const Span& sp : spans) n += grid_of(sp);
   int at = n;
   for (auto sp = spans.rbegin(); sp != spans.rend(); ++sp) {
     const int grid = grid_of(*sp);
     at -= grid;
-    with_table(tensors, *sp, [&](const auto& tab) { grad_squares_kernel<<<grid, kThreads, 0, s>>>(partial + at, tab); });
+    cudaError_t e = cudaSuccess;
+    with_table(tensors, *sp, [&](const auto& tab) { e = launch_squares_of(grid, s, partial + at, tab); });
+    LLMK_TRY(cuda_check(e, "grad_squares_kernel"));
     count_launch();
   }
-  return n;
+  *partials = n;
+  return LLMK_OK;
 }
 
 template <int kCap>
@@ -413,13 +423,12 @@ int grad_norm(float* norm, const llmk_tensor* tensors, int count, float scale, v
   const auto spans = spans_of(tensors, count);
   LLMK_TRY(check_workspace("grad_norm", spans, workspace, workspace_bytes));
   auto* partial = static_cast<double*>(workspace);
-  const int n = launch_squares(partial, tensors, spans, s);
+  int n = 0;
+  LLMK_TRY(launch_squares(&n, partial, tensors, spans, s));
   LLMK_CUDA(launch_after(grad_norm_kernel, 1, kThreads, 0, s, norm, partial, n, scale));
   count_launch();
-  LLMK_CUDA(cudaGetLastError());
   return LLMK_OK;
 }
-
 
 int clip_grad_norm(float* norm, const llmk_tensor* tensors, int count, float max_norm, void* workspace,
                    size_t workspace_bytes, cudaStream_t s) {
@@ -428,7 +437,8 @@ int clip_grad_norm(float* norm, const llmk_tensor* tensors, int count, float max
   const auto spans = spans_of(tensors, count);
   LLMK_TRY(check_workspace("clip_grad_norm", spans, workspace, workspace_bytes));
   auto* partial = static_cast<double*>(workspace);
-  const int n = launch_squares(partial, tensors, spans, s);
+  int n = 0;
+  LLMK_TRY(launch_squares(&n, partial, tensors, spans, s));
   // Many units: a block for each, in order, streams faster than a fixed grid that
   // walks them (124M bf16 gradients 128 -> 122 us, fp32 267 -> 237 us), but its
   // prologue cannot be the sum of the partials. Few: one launch less counts.
