@@ -326,7 +326,9 @@ int llmk_preference_loss(float* losses, float* rewards, float* logps, void* dlog
  * tensor cores, whose epilogue leaves each row's softmax statistics, so that the
  * logits are not read to find the losses; with backward != 0 one more pass
  * overwrites them with the gradient (0 in rows of weight 0). Arguments, outputs
- * and refusals as above; BT = 2 * pairs * T for the preference loss. The
+ * and refusals as above, but for a type of the logits that is neither fp32 nor
+ * bf16: an invalid argument here, as in llmk_matmul_crossentropy_forward. BT = 2 *
+ * pairs * T for the preference loss. The
  * statistics are those of the stored logits: with bf16 logits the
  * log-probabilities carry their rounding. workspace >=
  * llmk_matmul_finetune_workspace(BT, Vp). */

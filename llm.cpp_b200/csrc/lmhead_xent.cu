@@ -317,6 +317,7 @@ int llmk_matmul_policy_forward(float* losses, float* kls, float* logps, void* lo
                                llmk_math math, void* workspace, size_t workspace_bytes, void* stream) {
   const PolicyArgs a{losses, kls, logps, targets, weights, advantages, old_logps, ref_logps, clip_low, clip_high, kl_coef, dscale};
   LLMK_TRY(check_policy("matmul_policy", a, BT));
+  if (BT > (1 << 30)) return fail(LLMK_ERR_UNSUPPORTED, "matmul_policy: more than 2^30 rows");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   void* scratch = nullptr;
   LLMK_TRY(finetune_logits("matmul_policy", logits, dtype, inp, W, bias, BT, C, Vp, V, math, workspace, workspace_bytes, s,

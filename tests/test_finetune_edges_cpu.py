@@ -3,6 +3,8 @@ import os
 import subprocess
 import sys
 
+from test_finetune_cpu import UNSUPPORTED, matmul_policy, matmul_preference, policy, preference
+
 PKG = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "llm.cpp_b200")
 CUDA = 3
 
@@ -28,3 +30,13 @@ def test_a_refused_launch_ends_the_norm(llmk_lib):
     assert len(lines) == 2
     for line in lines:
         assert line.startswith("grad_squares_kernel: ") and line.endswith(" 0"), line
+
+
+def test_more_rows_than_the_losses_take(llmk_lib):
+    """Up to 2^30 rows, in every form."""
+    L, most = llmk_lib, 1 << 30
+    for f, args in ((L.llmk_policy_loss, policy(rows=most + 1)), (L.llmk_matmul_policy_forward, matmul_policy(BT=most + 1)),
+                    (L.llmk_preference_loss, preference(pairs=1, T=most // 2 + 1)),
+                    (L.llmk_matmul_preference_forward, matmul_preference(pairs=1, T=most // 2 + 1))):
+        assert f(*args) == UNSUPPORTED
+        assert b"more than 2^30 rows" in L.llmk_last_error()
