@@ -51,10 +51,10 @@ struct __align__(16) RowCoef {
   int target;
 };
 
-__device__ __forceinline__ float warp_max_f(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
+__device__ __forceinline__ float warp_max_f(float v) {  // of the values that are not NaN
+  float m;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
 }
 __device__ __forceinline__ float warp_sum_f(float v) {
 #pragma unroll
@@ -244,16 +244,20 @@ __device__ __forceinline__ float first_elem(const uint4& u) {
 
 // A warp's running maximum and sum of exp(x - m). m starts as the maximum over
 // the warp's first vectors and, in a lane, follows a value more than 10 above it:
-// the terms stay far inside fp32's range, and a lane that raises m is rare.
-// ex2.approx is 5e-8 low on average (measured), and one fp32 product by log2 e
-// moves a term by its distance times 1.3e-8. A sum over a vocabulary keeps the
-// mean of that while the rounding errors cancel, and a preference loss adds such
-// sums over a thousand positions. So one term in 8 to 32 is also computed by
-// expf, and the sum is corrected by what those terms differ by: the mean error
-// of a row's log-probability falls from 5e-8 to below 1e-8 for less than one more
-// instruction per element (evaluation of 8 x 1024 rows 165 against 169 us). The
+// the terms stay far inside fp32's range, and a lane that raises m is rare (at
+// every new maximum: evaluation of 8 x 1024 rows 137 against 131 us).
+// ex2.approx is 5e-8 low on average (measured), and the fp32 product by log2 e
+// moves a term by its distance from m times 1.3e-8. A sum over a vocabulary keeps
+// the mean of that while the rounding errors cancel, and a preference loss adds
+// such sums over a thousand positions. Two things hold that mean at 1.2e-8 of a
+// row's log-probability, for logits spread by 0.1 to 4 and for one that stands 2
+// to 15 above the others, in vocabularies of 1000 to 50257. The row's maximum is
+// taken out of its lane's sum at the end and counts exactly 1 (7e-8 with it left
+// in, where it stands out). And one term in 8 to 32 is also computed by expf, and
+// the sum of the others is corrected by what those terms differ by (1.9e-8
+// without; evaluation 131 against 126 us, the gradient 425 against 431 us). The
 // terms on the FMA units instead, by a polynomial, are as exact but slower: 185
-// against 174 us with an eighth of them there, 202 us with three eighths.
+// against 174 us (evaluation at that time) with an eighth of them there.
 struct WarpSum {
   float top, m, s;
   float part, off;  // the terms computed twice: their sum, and what it lacks
@@ -312,11 +316,14 @@ struct RunningSum {
     if (i < full) add<T>(x[i]);
     if (partial && lane == 0) add<T>(cut_vec<T>(x[full], keep));
   }
-  // The warp's sums, at one m.
-  __device__ __forceinline__ WarpSum join() const {
+  // The warp's sums, at one m, without the term of its maximum: a value up to 10
+  // above m had it off by up to 2e-7, while it is exp(top - m) to be joined.
+  __device__ __forceinline__ WarpSum join(int lane) const {
     float s0, s1;
     f2_unpack(s, s0, s1);
     WarpSum w{warp_max_f(top), m0, s0 + s1, part, off};
+    const unsigned holders = __ballot_sync(0xffffffffu, top == w.top);
+    if (lane == __ffs(holders) - 1) w.s -= ex2_approx((top - finite_max(m)) * kLog2e);  // as sum_exp_vec has it
     if (__any_sync(0xffffffffu, m != m0)) {  // also where m is NaN
       w.m = warp_max_f(m);
       const float f = expf(m - finite_max(w.m));
@@ -350,15 +357,15 @@ __device__ __forceinline__ WarpSum exact_sum(const uint4* x, int full, bool part
   return WarpSum{top, top, high, 0.f, static_cast<float>(s - static_cast<double>(high))};
 }
 
-// A row's sum from sums over its warps, at its maximum M. `off / part` is what
-// the terms lack; expf itself is 6e-9 high on average, in the terms computed
-// twice and in the warps' factors. The maximum's own term is exactly 1 and needs
-// no correction. No term is off by more than 2e-6, whatever its distance; a
-// larger quotient comes from terms that are next to nothing (where ex2.approx
-// flushes to zero and expf does not) and says nothing about the others.
-__device__ __forceinline__ RowSum corrected(float M, float sum, float part, float off) {
+// A row's sum at its maximum M: `tops` terms that are exactly 1, and the sum of all
+// others from terms of ex2.approx. `off / part` is what those lack; expf itself is
+// 6e-9 high on average, in the terms computed twice and in the warps' factors. No
+// term up to 25 below the reference is off by more than 5e-7; a larger quotient
+// comes from terms that are next to nothing (where ex2.approx flushes to zero and
+// expf does not) and says nothing about the others.
+__device__ __forceinline__ RowSum corrected(float M, int tops, float sum, float part, float off) {
   const double s = sum, lack = fminf(fmaxf(off / part, -2e-6f), 2e-6f);
-  return RowSum{part > 0.f ? s + (s - 1.0) * (lack - 1.2e-8) : s, M, 0.f};
+  return RowSum{tops + (part > 0.f ? s + s * (lack - 1.2e-8) : s), M, 0.f};
 }
 // A row's sum from one warp's, or from several (lanes >= count: none); the same
 // in every lane.
@@ -371,15 +378,17 @@ __device__ __forceinline__ RowSum fold_exact(const WarpSum* sums, int count, int
 }
 __device__ __forceinline__ RowSum fold_warp(const WarpSum& w) {
   const float f = expf(w.m - finite_max(w.top));
-  return corrected(w.top, w.s * f, w.part, w.off);
+  return corrected(w.top, w.top == -INFINITY ? 0 : 1, w.s * f, w.part, w.off);
 }
 __device__ __forceinline__ RowSum fold_warps(const WarpSum* sums, int count, int lane) {
   WarpSum w{-INFINITY, -INFINITY, 0.f, 0.f, 0.f};
   if (lane < count) w = sums[lane];
   const float M = warp_max_f(w.top);
   const float f = expf(w.m - finite_max(M));
-  const float S = warp_sum_f(w.s * f), P = warp_sum_f(w.part * f), D = warp_sum_f(w.off * f);
-  return corrected(M, S, P, D);
+  const int tops = M == -INFINITY ? 0 : __popc(__ballot_sync(0xffffffffu, w.top == M));
+  const float others = w.top == M ? 0.f : expf(w.top - M);
+  const float S = warp_sum_f(w.s * f + others), P = warp_sum_f(w.part * f), D = warp_sum_f(w.off * f);
+  return corrected(M, tops, S, P, D);
 }
 
 // -exp(x - max) scale over a vector: the gradient everywhere but at the target.
@@ -716,7 +725,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) row_kernel(T* dlogits, const T
         load_next();
       }
     }
-    if constexpr (!kExact) sum = run.join();
+    if constexpr (!kExact) sum = run.join(lane);
     // Two sets of sums: a set is rewritten two rows on, and between lies a
     // meeting that the group's first warp reaches only after reading it.
     if (G > 1 || kExact) {

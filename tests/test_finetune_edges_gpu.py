@@ -93,3 +93,66 @@ def test_policy_loss_and_gradient_take_the_same_branch(cuda_dev, shape):
     assert torch.equal(zero[~near], (past > 0)[~near])
     loss = -p.w.double() * p.A.double() * torch.where(past > 0, limit, rho)
     assert ((p.losses.double() - loss).abs() <= loss.abs() * (U + 2 * LEAN)).all()
+
+
+# The mean error of a long row's log-probability: expf's own mean of 6e-9 in the terms that correct the sum, and again in
+# the factors that join it.
+MEAN = 1.2e-8
+# The other part of it, which differs from row to row: the roundings of a warp's and of a group's joins, 10 of them of
+# u / sqrt(3) each (those of the lanes' sums average out over 32 lanes and more).
+SPREAD = 10 ** 0.5 * U / 3 ** 0.5
+
+
+def long_rows(rows, V, dt, dev, spread=0.0, peak=0.0, target_is_peak=False):
+    """Normal logits of a spread, or even ones with one token in each row that stands `peak` above them; targets, and
+    their log-probabilities in 64 bits."""
+    g = torch.Generator(device=dev)
+    g.manual_seed(rows + V)
+    x = torch.empty(rows, -(-V // 8) * 8, device=dev, dtype=dt)
+    t = torch.randint(0, V, (rows,), generator=g, device=dev, dtype=torch.int32)
+    lp = torch.empty(rows, dtype=torch.float64, device=dev)
+    for i in range(0, rows, 2048):
+        part, pt = x[i:i + 2048], t[i:i + 2048].long()[:, None]
+        if peak:
+            v = torch.rand(part.shape, generator=g, device=dev)
+            at = pt if target_is_peak else torch.randint(0, V, pt.shape, generator=g, device=dev)
+            v.scatter_(1, at, peak + torch.rand(pt.shape, generator=g, device=dev))
+        else:
+            v = torch.randn(part.shape, generator=g, device=dev) * spread
+        part.copy_(v)
+        v = part[:, :V].double()
+        lp[i:i + 2048] = v.gather(-1, pt)[:, 0] - torch.logsumexp(v, -1)
+    return x, t, lp
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,V,kw", [(16384, 1000, dict(spread=1.0)), (16384, 20000, dict(spread=1.0)), (16384, 4097, dict(spread=4.0)),
+                                    (16384, 20000, dict(peak=2.0)), (16384, 1000, dict(peak=10.0)), (8192, 4097, dict(peak=10.0)),
+                                    (4096, 50257, dict(peak=8.0))])
+def test_rewards_of_long_sequences_do_not_lean(cuda_dev, T, V, kw, dt):
+    """A reward adds its sequence's log-probabilities: the mean error counts T times, the others' sum grows by sqrt(T).
+    A row whose greatest logit stands out is off no more: that term is exactly 1, wherever it is met."""
+    import llmk
+    x, t, lp = long_rows(2 * T, V, dt, cuda_dev, **kw)
+    L = lp.view(2, T).sum(-1)
+    ref, rewards, loss = L.float(), torch.empty(2, device=cuda_dev), torch.empty(1, device=cuda_dev)
+    ws = torch.empty(llmk.preference_loss_workspace(1, T, x.shape[1]), dtype=torch.uint8, device=cuda_dev)
+    llmk.preference_loss(loss, x, t, V=V, ref_logps=ref, rewards=rewards, beta=1.0, workspace=ws)
+    want = L - ref.double()  # what rounding the reference leaves
+    assert ((rewards.double() - want).abs() <= T * MEAN + 6 * SPREAD * math.sqrt(T) + U * want.abs()).all()
+
+
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,V,peak", [(16384, 1000, 8.0), (16384, 4097, 10.0), (8192, 50257, 10.0)])
+def test_log_probabilities_of_confident_rows_do_not_lean(cuda_dev, rows, V, peak, dt, grad):
+    """The mean error of the policy loss's log-probabilities where the target stands out, to 5 standard deviations, the
+    results' own roundings (uniform in a step) among them."""
+    import llmk
+    x, t, lp = long_rows(rows, V, dt, cuda_dev, peak=peak, target_is_peak=True)
+    A, losses, logps = torch.ones(rows, device=cuda_dev), torch.empty(rows, device=cuda_dev), torch.empty(rows, device=cuda_dev)
+    ws = torch.empty(llmk.policy_loss_workspace(rows, x.shape[1]), dtype=torch.uint8, device=cuda_dev)
+    llmk.policy_loss(losses, x, t, A, V=V, logps=logps, dlogits=x if grad else None, workspace=ws)
+    step = 2.0 ** (torch.floor(torch.log2(lp.abs())) - 23)
+    var = (step.square() / 12).mean().item() + SPREAD ** 2
+    assert abs((logps.double() - lp).mean().item()) <= MEAN + 5 * math.sqrt(var / rows)
