@@ -1284,18 +1284,39 @@ int llmk_adamw_device_hparams(float* params, void* params_bf16, const float* gra
   return LLMK_OK;
 }
 
-int llmk_adamw_clipped(float* params, void* params_bf16, const float* grads, float* m, float* v, long long n,
-                       const float* hparams, const float* norm, float max_norm, void* stream) {
-  if (!params || !grads || !m || !v || n < 0 || !hparams || !norm || !(max_norm > 0.f))
+// hparams: in device memory, or nullptr for `now`.
+static int launch_adamw_clipped(float* params, void* params_bf16, const float* grads, float* m, float* v, long long n,
+                                const float* hparams, const AdamHP& now, const float* norm, float max_norm, cudaStream_t stream) {
+  if (!params || !grads || !m || !v || n < 0 || !norm || !(max_norm > 0.f))
     return fail(LLMK_ERR_INVALID_ARG, "adamw_clipped: null operand, or max_norm not above 0");
   if (n % 4 || !a16(params) || !a16(params_bf16) || !a16(grads) || !a16(m) || !a16(v) || !a16(hparams))
     return fail(LLMK_ERR_UNSUPPORTED, "adamw_clipped: n % 4 == 0 and 16-byte alignment required");
-  adamw_kernel<true><<<grid_for(n / 4, 256), 256, 0, static_cast<cudaStream_t>(stream)>>>(
-      params, static_cast<__nv_bfloat16*>(params_bf16), grads, m, v, n / 4, AdamHP{},
-      reinterpret_cast<const AdamHP*>(hparams), norm, max_norm);
+  adamw_kernel<true><<<grid_for(n / 4, 256), 256, 0, stream>>>(params, static_cast<__nv_bfloat16*>(params_bf16), grads, m, v,
+                                                              n / 4, now, reinterpret_cast<const AdamHP*>(hparams), norm,
+                                                              max_norm);
   count_launch();
   LLMK_CUDA(cudaGetLastError());
   return LLMK_OK;
 }
 
+int llmk_adamw_clipped(float* params, void* params_bf16, const float* grads, float* m, float* v, long long n,
+                       const float* hparams, const float* norm, float max_norm, void* stream) {
+  if (!hparams) return fail(LLMK_ERR_INVALID_ARG, "adamw_clipped: null operand, or max_norm not above 0");
+  return launch_adamw_clipped(params, params_bf16, grads, m, v, n, hparams, AdamHP{}, norm, max_norm,
+                              static_cast<cudaStream_t>(stream));
+}
+
 }  // extern "C"
+
+namespace llmk {
+
+int adamw_clipped(float* params, void* params_bf16, const float* grads, float* m, float* v, long long n, float lr, float beta1,
+                  float beta2, float eps, float weight_decay, int t, float grad_scale, const float* norm, float max_norm,
+                  cudaStream_t stream) {
+  float h[8];
+  llmk_adamw_hparams(h, lr, beta1, beta2, eps, weight_decay, t, grad_scale);
+  return launch_adamw_clipped(params, params_bf16, grads, m, v, n, nullptr,
+                              AdamHP{h[0], h[1], h[2], h[3], h[4], h[5], h[6], h[7]}, norm, max_norm, stream);
+}
+
+}  // namespace llmk

@@ -883,8 +883,8 @@ int llmk_gpt2_backward(llmk_gpt2* g) {
 // their bucket is — so that update overlaps the embedding all-reduce, the
 // one the backward cannot hide. With clipping on, the norm of all gradients comes
 // first and AdamW scales them on the way in. hp: the hyperparameters in device
-// memory (the form a captured graph replays, and clipping reads), or nullptr to
-// pass them by value.
+// memory (the form a captured graph replays), or nullptr to pass them by value (a
+// caller may capture llmk_gpt2_update: no copy from this call's stack).
 static int adamw_ranges(llmk_gpt2* g, const float* hp, float lr, float beta1, float beta2, float eps,
                         float weight_decay, int t) {
   const float scale = 1.0f / static_cast<float>(g->world);
@@ -893,9 +893,12 @@ static int adamw_ranges(llmk_gpt2* g, const float* hp, float lr, float beta1, fl
     TimedScope ts(g, KC_ADAMW, static_cast<double>(end - begin) * (28.0 + (g->params_bf16 ? 2.0 : 0.0)));
     __nv_bfloat16* pb = g->params_bf16 ? g->params_bf16 + begin : nullptr;
     const long long n = static_cast<long long>(end - begin);
-    if (g->max_norm > 0.f)
+    if (g->max_norm > 0.f && hp)
       return llmk_adamw_clipped(g->params + begin, pb, g->grads + begin, g->m + begin, g->v + begin, n, hp, g->grad_norm,
                                 g->max_norm, g->stream);
+    if (g->max_norm > 0.f)
+      return llmk::adamw_clipped(g->params + begin, pb, g->grads + begin, g->m + begin, g->v + begin, n, lr, beta1, beta2,
+                                 eps, weight_decay, t, scale, g->grad_norm, g->max_norm, g->stream);
     if (hp)
       return llmk_adamw_device_hparams(g->params + begin, pb, g->grads + begin, g->m + begin, g->v + begin, n, hp,
                                        g->stream);
@@ -953,12 +956,7 @@ int llmk_gpt2_grad_norm(llmk_gpt2* g, float* host_norm) {
 
 int llmk_gpt2_update(llmk_gpt2* g, float lr, float beta1, float beta2, float eps, float weight_decay, int t) {
   if (!g || t < 1) return fail(LLMK_ERR_INVALID_ARG, "gpt2_update");
-  if (g->max_norm > 0.f) {
-    LLMK_TRY(copy_hparams(g, lr, beta1, beta2, eps, weight_decay, t));
-    LLMK_TRY(update_device_hparams(g));
-  } else {
-    LLMK_TRY(adamw_ranges(g, nullptr, lr, beta1, beta2, eps, weight_decay, t));
-  }
+  LLMK_TRY(adamw_ranges(g, nullptr, lr, beta1, beta2, eps, weight_decay, t));
   ++g->steps;
   return LLMK_OK;
 }

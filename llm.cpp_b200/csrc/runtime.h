@@ -102,6 +102,10 @@ int logps_finish(float* logps, const void* logits, llmk_dtype dtype, const float
                  int ld, void* scratch, cudaStream_t stream);
 // *out = sum(x[0..n)) / div, in a fixed order.
 int sum_losses(float* out, const float* x, int n, float div, cudaStream_t stream);
+// llmk_adamw_clipped with the hyperparameters of llmk_adamw by value (elementwise.cu).
+int adamw_clipped(float* params, void* params_bf16, const float* grads, float* m, float* v, long long n, float lr, float beta1,
+                  float beta2, float eps, float weight_decay, int t, float grad_scale, const float* norm, float max_norm,
+                  cudaStream_t stream);
 // The refusals of the two losses' entry points (LLMK_OK when there is none).
 int check_policy(const char* what, const PolicyArgs& a, int rows);
 int check_preference(const char* what, const PreferenceArgs& a, int pairs, int T);
