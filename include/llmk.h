@@ -383,14 +383,15 @@ typedef struct llmk_tensor {
 /* *norm = |scale| * sqrt(sum of the squares of every element of `count`
  * tensors), in one launch for up to 1000 tensors and one more for the sum
  * (sums in 64 bits, in a fixed order). `tensors` is a host array, read during the call. workspace >=
- * llmk_grad_norm_workspace(). The reference has no counterpart: its trainer
+ * llmk_grad_norm_workspace(), apart from the tensors. The reference has no counterpart: its trainer
  * does not clip (gpt2/cuda/gpt2cuda.cu:420-459). */
 size_t llmk_grad_norm_workspace(const llmk_tensor* tensors, int count);
 int llmk_grad_norm(float* norm, const llmk_tensor* tensors, int count, float scale, void* workspace,
                    size_t workspace_bytes, void* stream);
 /* *norm as above (scale 1), then out = data * min(1, max_norm / (*norm +
  * 1e-6)) for every tensor, max_norm > 0. A norm that is not finite reaches the
- * outputs (inf: 0 or NaN, NaN: NaN). No written tensor may overlap another. */
+ * outputs (inf: 0 or NaN, NaN: NaN). No written tensor may overlap another, and no tensor
+ * norm or the workspace. */
 int llmk_clip_grad_norm(float* norm, const llmk_tensor* tensors, int count, float max_norm, void* workspace,
                         size_t workspace_bytes, void* stream);
 /* llmk_adamw_device_hparams with gradients clipped on the way in: they are

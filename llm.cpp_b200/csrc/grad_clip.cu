@@ -416,12 +416,36 @@ int no_throw(F f) {
   }
 }
 
+// Whether [p, p + bytes) meets a tensor that is read, or (writes) written.
+bool meets(const void* p, size_t bytes, const llmk_tensor* tensors, int count, bool writes) {
+  const uintptr_t begin = reinterpret_cast<uintptr_t>(p), end = begin + bytes;
+  auto meet = [&](const void* t, size_t n) {
+    const uintptr_t b = reinterpret_cast<uintptr_t>(t);
+    return n > 0 && begin < b + n && b < end;
+  };
+  for (int i = 0; i < count; ++i) {
+    const llmk_tensor& t = tensors[i];
+    if (meet(t.data, t.n * elem_size(t.dtype)) || (writes && meet(t.out, t.n * elem_size(t.out_dtype)))) return true;
+  }
+  return false;
+}
+
+// The partial sums are written while the tensors are read; clipping reads the norm
+// while it writes tensors.
+int check_scratch(const char* what, const float* norm, const void* workspace, size_t bytes, const llmk_tensor* tensors, int count,
+                  bool writes) {
+  if (meets(workspace, bytes, tensors, count, writes) || (writes && meets(norm, sizeof(float), tensors, count, true)))
+    return fail(LLMK_ERR_INVALID_ARG, std::string(what) + ": norm or workspace overlaps a tensor");
+  return LLMK_OK;
+}
+
 int grad_norm(float* norm, const llmk_tensor* tensors, int count, float scale, void* workspace, size_t workspace_bytes,
               cudaStream_t s) {
   if (!norm || !std::isfinite(scale)) return fail(LLMK_ERR_INVALID_ARG, "grad_norm: null norm or bad scale");
   LLMK_TRY(check_tensors("grad_norm", tensors, count, false));
   const auto spans = spans_of(tensors, count);
   LLMK_TRY(check_workspace("grad_norm", spans, workspace, workspace_bytes));
+  LLMK_TRY(check_scratch("grad_norm", norm, workspace, workspace_of(spans), tensors, count, false));
   auto* partial = static_cast<double*>(workspace);
   int n = 0;
   LLMK_TRY(launch_squares(&n, partial, tensors, spans, s));
@@ -436,6 +460,7 @@ int clip_grad_norm(float* norm, const llmk_tensor* tensors, int count, float max
   LLMK_TRY(check_tensors("clip_grad_norm", tensors, count, true));
   const auto spans = spans_of(tensors, count);
   LLMK_TRY(check_workspace("clip_grad_norm", spans, workspace, workspace_bytes));
+  LLMK_TRY(check_scratch("clip_grad_norm", norm, workspace, workspace_of(spans), tensors, count, true));
   auto* partial = static_cast<double*>(workspace);
   int n = 0;
   LLMK_TRY(launch_squares(&n, partial, tensors, spans, s));

@@ -3,7 +3,9 @@ import os
 import subprocess
 import sys
 
-from test_finetune_cpu import UNSUPPORTED, matmul_policy, matmul_preference, policy, preference
+import pytest
+
+from test_finetune_cpu import BF16, F32, INVALID, UNSUPPORTED, A, matmul_policy, matmul_preference, policy, preference, tensors
 
 PKG = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "llm.cpp_b200")
 CUDA = 3
@@ -18,6 +20,21 @@ for f in (L.llmk_grad_norm, L.llmk_clip_grad_norm):
     assert f(A, tensors, 1, 1.0, A, 1 << 30, None) == {cuda}
     print(L.llmk_last_error().decode(), L.llmk_launch_count())
 """
+
+FAR = A + (1 << 24)
+
+
+@pytest.mark.parametrize("norm,ws,clip_only", [
+    (A, FAR, True), (A + 396, FAR, True), (A + 8192, FAR, True), (A + 8192 + 196, FAR, True),  # the norm in a tensor, in an output
+    (FAR, A + 384, False), (FAR, A, False), (FAR, A + 4096, False),  # the workspace across one
+    (FAR, A + 8192 + 128, True),  # across an output only
+])
+def test_norm_and_workspace_inside_a_tensor(llmk_lib, norm, ws, clip_only):
+    L, t = llmk_lib, tensors((A, A, 100, F32, F32), (A + 4096, A + 8192, 100, BF16, BF16), (None, None, 0, F32, F32))
+    assert L.llmk_clip_grad_norm(norm, t, 3, 1.0, ws, 1 << 20, None) == INVALID
+    assert b"clip_grad_norm: norm or workspace overlaps" in L.llmk_last_error()
+    if not clip_only:  # the norm alone writes no tensor, and its result last
+        assert L.llmk_grad_norm(norm, t, 3, 1.0, ws, 1 << 20, None) == INVALID
 
 
 def test_a_refused_launch_ends_the_norm(llmk_lib):
