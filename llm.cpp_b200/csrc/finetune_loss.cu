@@ -10,12 +10,12 @@
 // Memory bounds both. The policy loss is independent from row to row, so one
 // kernel (row_kernel) reads each row once, keeps it in shared memory while its
 // sum forms, and writes the gradient from there: 16 x 1024 rows of 50257 bf16
-// logits, half of them live, in 418 us, 5.9 TB/s of the 2.47 GB it cannot do
+// logits, half of them live, in 425 us, 5.8 TB/s of the 2.47 GB it cannot do
 // without (a copy of the kernel without its arithmetic takes as long). The
 // preference loss needs the sums over whole sequences before the first gradient:
 // row_kernel leaves each row's (max, sum), preference_pair_kernel forms the
 // losses and every row's coefficient, and row_gradient_kernel streams the logits
-// a second time: 8 pairs of 1024 positions in 590 us, 5.6 TB/s of 3.30 GB. A few
+// a second time: 8 pairs of 1024 positions in 598 us, 5.5 TB/s of 3.30 GB. A few
 // long rows take that second way for the policy loss too. Of two variants that a
 // comment compares, both were measured with the rest of the kernel as it was then.
 #include <algorithm>

@@ -336,7 +336,8 @@ def preference_loss(losses, logits, targets, *, V=None, weights=None, ref_logps=
 
 class TensorList:
     """The gradient tensors that grad_norm and clip_grad_norm run over, and (outs, default: in place) where the
-    clipped ones go. Built once; it keeps the tensors alive."""
+    clipped ones go. It keeps the tensors alive and reads their addresses once, here: build it once for gradients that
+    stay where they are (some 2 us a tensor), and again for gradients that are allocated anew."""
 
     def __init__(self, tensors, outs=None):
         self.tensors = list(tensors)
