@@ -390,8 +390,8 @@ int llmk_grad_norm(float* norm, const llmk_tensor* tensors, int count, float sca
                    size_t workspace_bytes, void* stream);
 /* *norm as above (scale 1), then out = data * min(1, max_norm / (*norm +
  * 1e-6)) for every tensor, max_norm > 0. A norm that is not finite reaches the
- * outputs (inf: 0 or NaN, NaN: NaN). No written tensor may overlap another, and no tensor
- * norm or the workspace. */
+ * outputs (inf: 0 or NaN, NaN: NaN). No written tensor may overlap another, no tensor
+ * norm or the workspace, and norm not the workspace. */
 int llmk_clip_grad_norm(float* norm, const llmk_tensor* tensors, int count, float max_norm, void* workspace,
                         size_t workspace_bytes, void* stream);
 /* llmk_adamw_device_hparams with gradients clipped on the way in: they are

@@ -431,11 +431,15 @@ bool meets(const void* p, size_t bytes, const llmk_tensor* tensors, int count, b
 }
 
 // The partial sums are written while the tensors are read; clipping reads the norm
-// while it writes tensors.
+// while it writes tensors, and its first block writes it while the others read the
+// partial sums.
 int check_scratch(const char* what, const float* norm, const void* workspace, size_t bytes, const llmk_tensor* tensors, int count,
                   bool writes) {
   if (meets(workspace, bytes, tensors, count, writes) || (writes && meets(norm, sizeof(float), tensors, count, true)))
     return fail(LLMK_ERR_INVALID_ARG, std::string(what) + ": norm or workspace overlaps a tensor");
+  const uintptr_t n = reinterpret_cast<uintptr_t>(norm), w = reinterpret_cast<uintptr_t>(workspace);
+  if (writes && n < w + bytes && w < n + sizeof(float))
+    return fail(LLMK_ERR_INVALID_ARG, std::string(what) + ": norm overlaps the workspace");
   return LLMK_OK;
 }
 

@@ -17,7 +17,7 @@ import llmk
 L, A = llmk.lib(), 1 << 20
 tensors = (llmk.Tensor * 1)(llmk.Tensor(None, None, 0, 0, 0))
 for f in (L.llmk_grad_norm, L.llmk_clip_grad_norm):
-    assert f(A, tensors, 1, 1.0, A, 1 << 30, None) == {cuda}
+    assert f(A, tensors, 1, 1.0, A + 64, 1 << 30, None) == {cuda}
     print(L.llmk_last_error().decode(), L.llmk_launch_count())
 """
 
@@ -35,6 +35,13 @@ def test_norm_and_workspace_inside_a_tensor(llmk_lib, norm, ws, clip_only):
     assert b"clip_grad_norm: norm or workspace overlaps" in L.llmk_last_error()
     if not clip_only:  # the norm alone writes no tensor, and its result last
         assert L.llmk_grad_norm(norm, t, 3, 1.0, ws, 1 << 20, None) == INVALID
+
+
+def test_norm_inside_the_workspace(llmk_lib):
+    L, t = llmk_lib, tensors((A, A, 20000, F32, F32))  # three units: three partial sums of 8 bytes
+    for norm in (FAR, FAR + 12, FAR + 20):
+        assert L.llmk_clip_grad_norm(norm, t, 1, 1.0, FAR, 1 << 20, None) == INVALID
+        assert b"clip_grad_norm: norm overlaps the workspace" in L.llmk_last_error()
 
 
 def test_a_refused_launch_ends_the_norm(llmk_lib):
